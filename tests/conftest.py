@@ -57,3 +57,11 @@ def mean_rel_err(a, b):
 
 
 GOLDEN_CASES = ["tiny_glu", "tiny_specials", "tiny_softmax", "tiny_raw", "e64_k6_fp32"]
+
+
+def pytest_collection_modifyitems(items):
+    # tests that need a checkout of the reference skip where its folder is there but empty (an unpopulated mount)
+    for item in items:
+        ref = getattr(item.module, "REF", None)
+        if ref is not None and ref.exists() and not (ref / "src").exists() and item.get_closest_marker("skipif"):
+            item.add_marker(pytest.mark.skip(reason="the reference folder holds no checkout"))
