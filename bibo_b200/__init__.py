@@ -2,8 +2,11 @@
 the reference's PyTorch module API.  See include/bibo_moe.h for the C ABI underneath."""
 from .moe import BiBoFusedExperts, BiBoMoELayer, BiBoMoERouter, MoEConfig  # noqa: F401
 from .mlp import BiBoMLP  # noqa: F401
+from .norm import BiBoLayerNorm, layer_norm  # noqa: F401
+from .dispatch import combine_tokens, dispatch_tokens  # noqa: F401
 from .trace import RouterTrace  # noqa: F401
 from . import functional  # noqa: F401
 from .install import install, uninstall  # noqa: F401
 
-__all__ = ["BiBoMoELayer", "BiBoMoERouter", "BiBoFusedExperts", "BiBoMLP", "MoEConfig", "RouterTrace", "functional", "install", "uninstall"]
+__all__ = ["BiBoMoELayer", "BiBoMoERouter", "BiBoFusedExperts", "BiBoMLP", "BiBoLayerNorm", "MoEConfig", "RouterTrace",
+           "layer_norm", "dispatch_tokens", "combine_tokens", "functional", "install", "uninstall"]

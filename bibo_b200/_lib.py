@@ -134,6 +134,18 @@ SIGNATURES = {
     "bibo_moe_rmsnorm_fwd": (_i32, [_vp, _vp, _f32, _i64, _i32, _i32, _vp, _vp]),
     "bibo_moe_rmsnorm_bwd_parts": (_i64, [_i64]),
     "bibo_moe_rmsnorm_bwd": (_i32, [_vp, _vp, _vp, _f32, _i64, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "bibo_moe_layernorm_fwd": (_i32, [_vp, _i64, _vp, _vp, _f32, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "bibo_moe_layernorm_bwd_parts": (_i64, [_i64]),
+    "bibo_moe_layernorm_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "bibo_moe_dispatch_rows_cap": (_i64, [_i64, _i32, _i32, _i32]),
+    "bibo_moe_dispatch_plan_words": (_i64, [_i64, _i32, _i32, _i32]),
+    "bibo_moe_dispatch_off_slot_row": (_i64, [_i32]),
+    "bibo_moe_dispatch_off_row_slot": (_i64, [_i64, _i32, _i32]),
+    "bibo_moe_dispatch_plan": (_i32, [_vp, _i32, _i64, _i32, _i32, _i32, _vp, _vp]),
+    "bibo_moe_dispatch_fwd": (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "bibo_moe_dispatch_combine_fwd": (_i32, [_vp, _vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "bibo_moe_dispatch_combine_bwd": (_i32, [_vp, _i64, _vp, _vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp,
+                                             _vp]),
     "bibo_moe_mlp_plan_words": (_i64, [_i64]),
     "bibo_moe_mlp_supported": (_i32, [_i32, _i32, _i32]),
     "bibo_moe_mlp_forward": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),

@@ -419,6 +419,127 @@ def experts_forward(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tenso
     return out, ws
 
 
+class DispatchPlan:
+    """Row order of one routing (bibo_moe_dispatch_plan): the slots of ``topk_idx`` sorted by expert, in slot order within
+    an expert.  ``rows`` is the number of rows of an expert-ordered buffer (a bound that the host knows); the device knows
+    how many of them are used.
+
+    * ``offsets`` int32 [E+1]: first row of each expert (a multiple of ``align``) and the row behind the last group
+    * ``counts`` int32 [E]: slots of each expert
+    * ``slot_row`` int32 [N,k]: row of a slot, -1 for an empty slot
+    * ``row_slot`` int32 [rows]: slot ``t*k + j`` of a row, -1 for a row without one
+    """
+
+    def __init__(self, n_tokens: int, top_k: int, n_experts: int, align: int, device):
+        lib = _lib.load()
+        self.n_tokens, self.top_k, self.n_experts, self.align = n_tokens, top_k, n_experts, align
+        self.rows = int(lib.bibo_moe_dispatch_rows_cap(n_tokens, top_k, n_experts, align))
+        if self.rows < 0:
+            raise RuntimeError("dispatch plan: " + lib.bibo_moe_last_error_string().decode(errors="replace"))
+        self.buf = torch.empty(int(lib.bibo_moe_dispatch_plan_words(n_tokens, top_k, n_experts, align)), dtype=torch.int32,
+                               device=device)
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        return self.buf[:self.n_experts + 1]
+
+    @property
+    def counts(self) -> torch.Tensor:
+        return self.buf[self.n_experts + 1:2 * self.n_experts + 1]
+
+    @property
+    def slot_row(self) -> torch.Tensor:
+        o = int(_lib.load().bibo_moe_dispatch_off_slot_row(self.n_experts))
+        return self.buf[o:o + self.n_tokens * self.top_k].view(self.n_tokens, self.top_k)
+
+    @property
+    def row_slot(self) -> torch.Tensor:
+        o = int(_lib.load().bibo_moe_dispatch_off_row_slot(self.n_tokens, self.top_k, self.n_experts))
+        return self.buf[o:o + self.rows]
+
+    def raise_if_failed(self) -> None:
+        """Waits for the plan and raises RuntimeError if an expert index was out of range (such slots count as empty)."""
+        code = int(self.buf[2 * self.n_experts + 1])
+        if code != 0:
+            raise RuntimeError(f"bibo_b200: the dispatch plan reported device status {code} ({STATUS_TEXT[code]})")
+
+
+def dispatch_plan(topk_idx: torch.Tensor, n_experts: int, align: int = 1) -> DispatchPlan:
+    """Row order of the routing ``topk_idx`` [N,k] (int32 or int64; a negative index is an empty slot, an expert may occur
+    more than once in a token).  ``align``: groups start at multiples of it, with rows without a slot behind them.  k up to
+    32, up to 1024 experts, one kernel launch, nothing is read back."""
+    _need_cuda(topk_idx, "topk_idx")
+    if topk_idx.dim() != 2 or topk_idx.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"topk_idx must be int32 or int64 [N, k], got {topk_idx.dtype} {tuple(topk_idx.shape)}")
+    n, k = topk_idx.shape
+    plan = DispatchPlan(n, k, int(n_experts), int(align), topk_idx.device)
+    _launch("bibo_moe_dispatch_plan", topk_idx.device, _lib.ptr(topk_idx), topk_idx.element_size(), n, k, plan.n_experts,
+            plan.align, _lib.ptr(plan.buf))
+    return plan
+
+
+def _need_plan_rows(t: torch.Tensor, name: str, plan: DispatchPlan, rows: int) -> None:
+    _need_rows(t, name)
+    if t.shape[0] != rows:
+        raise RuntimeError(f"{name} has {t.shape[0]} rows, the plan needs {rows}")
+    if t.device != plan.buf.device:
+        raise RuntimeError(f"{name} is on {t.device}, the plan on {plan.buf.device}")
+
+
+def _need_weights(topk_w: Optional[torch.Tensor], plan: DispatchPlan) -> int:
+    if topk_w is None:
+        return _lib.F32
+    _need_cuda(topk_w, "topk_w")
+    if topk_w.shape != (plan.n_tokens, plan.top_k) or topk_w.device != plan.buf.device:
+        raise RuntimeError(f"topk_w must be [{plan.n_tokens}, {plan.top_k}] on {plan.buf.device}, got "
+                           f"{tuple(topk_w.shape)} on {topk_w.device}")
+    return dtype_code(topk_w.dtype)
+
+
+def dispatch_forward(x: torch.Tensor, plan: DispatchPlan) -> torch.Tensor:
+    """Token rows x [N,H] in expert order (bibo_moe_dispatch_fwd): xs [plan.rows, H]; rows without a slot are zero."""
+    _need_plan_rows(x, "x", plan, plan.n_tokens)
+    dt = dtype_code(x.dtype)
+    xs = torch.empty((plan.rows, x.shape[1]), dtype=x.dtype, device=x.device)
+    _launch("bibo_moe_dispatch_fwd", x.device, _lib.ptr(x), x.stride(0), _lib.ptr(plan.buf), plan.n_tokens, x.shape[1],
+            plan.top_k, plan.n_experts, plan.align, dt, _lib.ptr(xs))
+    return xs
+
+
+def combine_forward(ys: torch.Tensor, topk_w: Optional[torch.Tensor], plan: DispatchPlan) -> torch.Tensor:
+    """out[t] = sum over the slots of t of topk_w[t,j] * ys[row of the slot] (bibo_moe_dispatch_combine_fwd), summed in fp32
+    in slot order.  ``topk_w`` [N,k] is fp32 or bf16, None for a plain sum; an empty slot's weight is not read."""
+    _need_plan_rows(ys, "ys", plan, plan.rows)
+    _need_cuda(ys, "ys")
+    dt, wt = dtype_code(ys.dtype), _need_weights(topk_w, plan)
+    out = torch.empty((plan.n_tokens, ys.shape[1]), dtype=ys.dtype, device=ys.device)
+    _launch("bibo_moe_dispatch_combine_fwd", ys.device, _lib.ptr(ys), _lib.ptr(topk_w), wt, _lib.ptr(plan.buf), plan.n_tokens,
+            ys.shape[1], plan.top_k, plan.n_experts, plan.align, dt, _lib.ptr(out))
+    return out
+
+
+def combine_backward(dout: torch.Tensor, ys: torch.Tensor, topk_w: Optional[torch.Tensor], plan: DispatchPlan,
+                     need_dw: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Gradients of ``combine_forward`` (bibo_moe_dispatch_combine_bwd): (dys [plan.rows, H] with zeros in the rows without a
+    slot, d_topk_w [N,k] in topk_w's dtype or None)."""
+    _need_plan_rows(dout, "dout", plan, plan.n_tokens)
+    _need_plan_rows(ys, "ys", plan, plan.rows)
+    _need_cuda(ys, "ys")
+    _need_rows(dout, "dout", ys.shape[1], ys)
+    dt, wt = dtype_code(ys.dtype), _need_weights(topk_w, plan)
+    dys = torch.empty_like(ys)
+    dw = torch.empty_like(topk_w) if need_dw and topk_w is not None else None
+    p = _lib.ptr
+    _launch("bibo_moe_dispatch_combine_bwd", ys.device, p(dout), dout.stride(0), p(ys), p(topk_w), wt, p(plan.buf),
+            plan.n_tokens, ys.shape[1], plan.top_k, plan.n_experts, plan.align, dt, p(dys), p(dw))
+    return dys, dw
+
+
+def dispatch_backward(dxs: torch.Tensor, plan: DispatchPlan) -> torch.Tensor:
+    """Gradient of ``dispatch_forward``: dx[t] = sum over the slots of t of dxs[row of the slot], in fp32 in slot order."""
+    return combine_forward(dxs, None, plan)
+
+
 def rmsnorm_forward(h: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
     """BiBoRMSNorm.forward on flat rows h [N,H] (bibo_moe_rmsnorm_fwd)."""
     lib = _lib.load()
@@ -448,6 +569,90 @@ def rmsnorm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, ep
                                         dtype_code(h.dtype), p(dh), p(partial), p(dweight), _stream(h.device)),
                "bibo_moe_rmsnorm_bwd")
     return dh, dweight
+
+
+def _need_rows(t: torch.Tensor, name: str, hidden: Optional[int] = None, like: Optional[torch.Tensor] = None) -> None:
+    """Rows [N,H] on a CUDA device whose elements are next to each other; the rows themselves may be further apart."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} is on {t.device}: the bibo_b200 kernels run only on CUDA devices "
+                           "(there is no CPU implementation)")
+    if t.dim() != 2 or t.shape[1] < 1:
+        raise RuntimeError(f"{name} must be rows [N, H] with H >= 1, got shape {tuple(t.shape)}")
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise RuntimeError(f"{name} must be contiguous within its rows, which may not overlap (strides {t.stride()})")
+    if hidden is not None and t.shape[1] != hidden:
+        raise RuntimeError(f"{name} has rows of {t.shape[1]} elements, expected {hidden}")
+    if like is not None:
+        _need_like(t, name, like)
+
+
+def _need_like(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+    if t.dtype != like.dtype:
+        raise RuntimeError(f"{name} dtype {t.dtype} != activation dtype {like.dtype}")
+    if t.device != like.device:
+        raise RuntimeError(f"{name} is on {t.device}, the activations on {like.device}")
+
+
+def _launch(name: str, dev: torch.device, *args) -> None:
+    """One C-ABI call on ``dev``'s current stream, with ``dev`` made current for it where another device is."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    _lib.check(rc, name)
+
+
+def layernorm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                      eps: float = 1e-5, keep: bool = False):
+    """Layer norm of flat rows x [N,H] over H (bibo_moe_layernorm_fwd): ``(x - mean) * rstd * weight + bias``, computed in
+    fp32 and rounded once.  The rows may be a slice of a wider tensor.  ``weight`` and ``bias`` [H] are each optional and
+    share one dtype, fp32 or that of x.  ``keep=True`` returns ``(out, saved)`` with what ``layernorm_backward`` needs."""
+    _need_rows(x, "x")
+    n, hidden = x.shape
+    wtype = x.dtype
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        _need_cuda(t, name)
+        if t.shape != (hidden,) or t.device != x.device:
+            raise RuntimeError(f"{name} must be [{hidden}] on {x.device}, got {tuple(t.shape)} on {t.device}")
+        if t.dtype not in (x.dtype, torch.float32) or (t is bias and weight is not None and bias.dtype != weight.dtype):
+            raise RuntimeError(f"{name} dtype {t.dtype}: weight and bias are both float32 or both {x.dtype}")
+        wtype = t.dtype
+    out = torch.empty((n, hidden), dtype=x.dtype, device=x.device)
+    stats = torch.empty((2, n), dtype=torch.float32, device=x.device) if keep else None
+    p = _lib.ptr
+    mean = p(stats)
+    _launch("bibo_moe_layernorm_fwd", x.device, p(x), x.stride(0), p(weight), p(bias), float(eps), n, hidden,
+            dtype_code(x.dtype), dtype_code(wtype), p(out), mean, None if stats is None else mean + 4 * n)
+    return (out, (stats, wtype)) if keep else out
+
+
+def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], saved, has_bias: bool = True,
+                       need_dweight: bool = True):
+    """Gradients of ``layernorm_forward(..., keep=True)`` (bibo_moe_layernorm_bwd): (dx [N,H], dweight [H] or None without
+    a weight, dbias [H] or None without a bias).  The sums over the rows are taken in a fixed order."""
+    stats, wtype = saved
+    _need_rows(x, "x")
+    n, hidden = x.shape
+    _need_rows(dy, "dy", hidden, x)
+    if dy.shape[0] != n or stats.shape != (2, n):
+        raise RuntimeError(f"dy has {dy.shape[0]} rows and the forward kept {stats.shape[1]}, x has {n}")
+    dev = x.device
+    dx = torch.empty((n, hidden), dtype=x.dtype, device=dev)
+    make = torch.empty if n else torch.zeros                   # sums over no rows
+    dweight = make(hidden, dtype=wtype, device=dev) if weight is not None and need_dweight else None
+    dbias = make(hidden, dtype=wtype, device=dev) if has_bias else None
+    partial = None
+    if dweight is not None or dbias is not None:
+        parts = int(_lib.load().bibo_moe_layernorm_bwd_parts(n))
+        partial = torch.empty((parts, 2, hidden), dtype=torch.float32, device=dev)
+    p = _lib.ptr
+    _launch("bibo_moe_layernorm_bwd", dev, p(x), x.stride(0), p(dy), dy.stride(0), p(weight), p(stats), p(stats) + 4 * n, n,
+            hidden, dtype_code(x.dtype), dtype_code(wtype), p(dx), p(partial), p(dweight), p(dbias))
+    return dx, dweight, dbias
 
 
 def mlp_forward(x: torch.Tensor, gate_proj: torch.Tensor, up_proj: torch.Tensor, down_proj: torch.Tensor,

@@ -347,9 +347,12 @@ def ffn_forward(decoder_layer, hidden_states: torch.Tensor) -> torch.Tensor:
     feed-forward block and the residual add.  Inference runs the norm kernel and folds the residual add
     into the combine kernel; with gradients on, norm and block run through their autograd nodes (kernels
     in both directions) and the residual add is torch's.  Written against the reference's attribute
-    names (``post_attention_layernorm``, ``mlp``, ``_bf16_moe_out``, ``_bf16_stream``)."""
+    names (``post_attention_layernorm``, ``mlp``, ``_bf16_moe_out``, ``_bf16_stream``).  A norm that is a
+    ``torch.nn.LayerNorm`` runs on the layer norm kernels, in both directions."""
     from .mlp import mlp_module_forward
+    from .norm import layer_norm_module_forward
     mlp, norm = decoder_layer.mlp, decoder_layer.post_attention_layernorm
+    is_layer_norm = isinstance(norm, nn.LayerNorm)
     is_moe = hasattr(mlp, "gate") and hasattr(mlp, "experts")
     block = (lambda x, res=None: layer_forward(mlp, x, res)) if is_moe else (lambda x, res=None: mlp_module_forward(mlp, x))
     bf16_out = bool(getattr(decoder_layer, "_bf16_moe_out", False))
@@ -359,7 +362,9 @@ def ffn_forward(decoder_layer, hidden_states: torch.Tensor) -> torch.Tensor:
     plain = hidden_states.dtype == torch.bfloat16 or not (bf16_out or bf16_stream)   # the casts are no-ops
     if needs_grad or not plain:
         shape = hidden_states.shape
-        if hidden_states.is_cuda and norm.weight.dtype == hidden_states.dtype:
+        if is_layer_norm:
+            x = layer_norm_module_forward(norm, hidden_states)
+        elif hidden_states.is_cuda and norm.weight.dtype == hidden_states.dtype:
             x = _RMSNormFunction.apply(hidden_states.reshape(-1, shape[-1]).contiguous(), norm.weight,
                                        norm.variance_epsilon).view(shape)
         else:
@@ -370,10 +375,13 @@ def ffn_forward(decoder_layer, hidden_states: torch.Tensor) -> torch.Tensor:
         hidden_states = hidden_states + out
         return hidden_states.to(torch.bfloat16) if bf16_stream else hidden_states
     shape = hidden_states.shape
-    if is_moe and fused_ffn_applies(mlp, hidden_states, norm):
+    if is_moe and not is_layer_norm and fused_ffn_applies(mlp, hidden_states, norm):
         return layer_forward(mlp, hidden_states, fused_norm=(norm.weight, float(norm.variance_epsilon)))
-    flat = hidden_states.reshape(-1, shape[-1]).contiguous()
-    x = Fn.rmsnorm_forward(flat, norm.weight, norm.variance_epsilon).view(shape)
+    if is_layer_norm:
+        x = layer_norm_module_forward(norm, hidden_states)
+    else:
+        flat = hidden_states.reshape(-1, shape[-1]).contiguous()
+        x = Fn.rmsnorm_forward(flat, norm.weight, norm.variance_epsilon).view(shape)
     if is_moe:
         return block(x, hidden_states)
     return mlp_module_forward(mlp, x, residual=hidden_states)     # the add happens in the down kernel's epilogue

@@ -546,6 +546,51 @@ int64_t bibo_moe_rmsnorm_bwd_parts(int64_t n_rows);
 int bibo_moe_rmsnorm_bwd(const void* h, const void* weight, const void* dy, float eps, int64_t n_rows,
                          int hidden, int dtype, void* dh, float* partial, void* dweight, void* stream);
 
+/* ---- layer norm ----------------------------------------------------------------------------------------
+ * No counterpart in the reference, whose blocks use RMSNorm: for blocks that put a layer norm in front of the same
+ * feed-forward path.  out = (x - mean) * rstd * weight + bias over each row, rstd = 1/sqrt(var + eps), computed in
+ * fp32 and rounded once.  x [N,H] with rows x_stride elements apart (any alignment; 16-byte aligned rows run faster),
+ * out [N,H] contiguous; weight / bias [H] or NULL, both of wdtype = dtype or float32.  mean / rstd [N] fp32, both or
+ * neither NULL: what the backward reads.                                                                 */
+int bibo_moe_layernorm_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias, float eps,
+                           int64_t n_rows, int hidden, int dtype, int wdtype, void* out, float* mean, float* rstd,
+                           void* stream);
+/* dx [N,H] contiguous, dweight / dbias [H] in wdtype (either NULL: not wanted); partial is fp32 scratch
+ * [bibo_moe_layernorm_bwd_parts(N), 2, H].  Deterministic (no float atomics).  n_rows == 0 writes nothing. */
+int64_t bibo_moe_layernorm_bwd_parts(int64_t n_rows);
+int bibo_moe_layernorm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
+                           const float* mean, const float* rstd, int64_t n_rows, int hidden, int dtype, int wdtype,
+                           void* dx, float* partial, void* dweight, void* dbias, void* stream);
+
+/* ---- tokens sorted by expert and back, for the caller's own experts ----------------------------------------
+ * The permute and the combine of the block (src/modeling/ffn/moe.py:56-82,93-101) as operators of their own, with
+ * gradients: rows of a group follow each other without tile padding (groups start at multiples of `align`, 1..1024),
+ * k <= 32, E <= 1024, an expert may occur twice in a token, a negative index is an empty slot (no row, weight not
+ * read, its gradient 0).  An index >= E counts as empty and raises the status word plan[2E+1] = 2.
+ * plan (bibo_moe_dispatch_plan_words int32): offsets [E+1], counts [E], status; from _off_slot_row: slot_row [N*k]
+ * (-1: empty slot); from _off_row_slot: row_slot [rows_cap] (-1: row without a slot).  Every word that a kernel reads
+ * is written by bibo_moe_dispatch_plan.  Expert-ordered buffers have bibo_moe_dispatch_rows_cap rows; the helpers
+ * return -1 for arguments out of range.  Hidden sizes, row strides (elements) and alignments are free.   */
+int64_t bibo_moe_dispatch_rows_cap(int64_t n_tokens, int top_k, int n_experts, int align);
+int64_t bibo_moe_dispatch_plan_words(int64_t n_tokens, int top_k, int n_experts, int align);
+int64_t bibo_moe_dispatch_off_slot_row(int n_experts);
+int64_t bibo_moe_dispatch_off_row_slot(int64_t n_tokens, int top_k, int n_experts);
+/* topk_idx [N,k], idx_bytes 4 or 8.                                                                       */
+int bibo_moe_dispatch_plan(const void* topk_idx, int idx_bytes, int64_t n_tokens, int top_k, int n_experts, int align,
+                           int32_t* plan, void* stream);
+/* xs[slot_row[t,j]] = x[t], rows without a slot zero.                                                    */
+int bibo_moe_dispatch_fwd(const void* x, int64_t x_stride, const int32_t* plan, int64_t n_tokens, int hidden, int top_k,
+                          int n_experts, int align, int dtype, void* xs, void* stream);
+/* out[t] = sum_j topk_w[t,j] * ys[slot_row[t,j]] in fp32, slot order; topk_w NULL: weights of 1, which is the gradient
+ * of bibo_moe_dispatch_fwd.  w_dtype: float32 or bfloat16.                                               */
+int bibo_moe_dispatch_combine_fwd(const void* ys, const void* topk_w, int w_dtype, const int32_t* plan, int64_t n_tokens,
+                                  int hidden, int top_k, int n_experts, int align, int dtype, void* out, void* stream);
+/* dys[slot_row[t,j]] = topk_w[t,j] * dout[t], rows without a slot zero; d_topk_w[t,j] = <ys row, dout[t]> in w_dtype
+ * (NULL: not wanted).                                                                                     */
+int bibo_moe_dispatch_combine_bwd(const void* dout, int64_t dout_stride, const void* ys, const void* topk_w, int w_dtype,
+                                  const int32_t* plan, int64_t n_tokens, int hidden, int top_k, int n_experts, int align,
+                                  int dtype, void* dys, void* d_topk_w, void* stream);
+
 /* ---- dense SwiGLU MLP -----------------------------------------------------------------------------
  * Replaces BiBoMLP.forward, `down_proj(act_fn(gate_proj(x)) * up_proj(x))` with act = SiLU
  * (src/modeling/ffn/mlp.py:33-34): the shared expert of the MoE layer (src/modeling/ffn/moe.py:120-127,
