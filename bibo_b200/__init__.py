@@ -4,9 +4,10 @@ from .moe import BiBoFusedExperts, BiBoMoELayer, BiBoMoERouter, MoEConfig  # noq
 from .mlp import BiBoMLP  # noqa: F401
 from .norm import BiBoLayerNorm, layer_norm  # noqa: F401
 from .dispatch import combine_tokens, dispatch_tokens  # noqa: F401
+from .muon import Muon  # noqa: F401
 from .trace import RouterTrace  # noqa: F401
 from . import functional  # noqa: F401
 from .install import install, uninstall  # noqa: F401
 
 __all__ = ["BiBoMoELayer", "BiBoMoERouter", "BiBoFusedExperts", "BiBoMLP", "BiBoLayerNorm", "MoEConfig", "RouterTrace",
-           "layer_norm", "dispatch_tokens", "combine_tokens", "functional", "install", "uninstall"]
+           "layer_norm", "dispatch_tokens", "combine_tokens", "Muon", "functional", "install", "uninstall"]

@@ -146,6 +146,8 @@ SIGNATURES = {
     "bibo_moe_dispatch_combine_fwd": (_i32, [_vp, _vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
     "bibo_moe_dispatch_combine_bwd": (_i32, [_vp, _i64, _vp, _vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp,
                                              _vp]),
+    "bibo_moe_orthogonalize_workspace": (_i64, [_i64, _i32, _i32]),
+    "bibo_moe_orthogonalize": (_i32, [_vp, _i64, _i64, _i32, _i32, _i64, _i32, _i32, _vp, _f32, _vp, _vp, _vp]),
     "bibo_moe_mlp_plan_words": (_i64, [_i64]),
     "bibo_moe_mlp_supported": (_i32, [_i32, _i32, _i32]),
     "bibo_moe_mlp_forward": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),

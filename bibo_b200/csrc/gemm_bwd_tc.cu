@@ -22,7 +22,6 @@ namespace tc {
 constexpr int MODE_DX = 0, MODE_DW = 1;
 constexpr int XBN = 256, XSTAGES = 4;
 constexpr int XB_BYTES = XBN * BK * 2;
-constexpr int MN_BOX = 64 * BK * 2;   // one [64 k-rows x 128 B] box
 
 struct XLayout {
   static constexpr int OFF_A = 0;
@@ -31,15 +30,6 @@ struct XLayout {
   static constexpr int OFF_BAR = OFF_C + 2 * C_SUB;
   static constexpr int BYTES = OFF_BAR + 256 + 1024;
 };
-
-__device__ __forceinline__ uint64_t make_sdesc_mn128(uint32_t smem_addr) {
-  uint64_t d = (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)(MN_BOX >> 4) << 16;   // leading byte offset: next 64 elements along M/N
-  d |= (uint64_t)(1024 >> 4) << 32;     // stride byte offset: next 8 k-rows
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
 
 struct BwdWork {
   int e, row0, m0, n0, k_blocks, krow0;

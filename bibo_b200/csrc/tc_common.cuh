@@ -101,6 +101,18 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* m, const void* s
                ::"l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(smem_src)), "r"(x), "r"(y)
                : "memory");
 }
+// the same on a 3-D map (x, row, matrix of a batch)
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, const void* smem_src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(smem_src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
 __device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
@@ -153,6 +165,10 @@ __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.
 // Instruction descriptor: bf16 x bf16 -> fp32, both operands K-major, M x N tile.
 __host__ __device__ constexpr uint32_t make_idesc_bf16(int M, int N) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// The same for f16 x f16 -> fp32 (both operand types are 0 in their fields).
+__host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 // Shared-memory matrix descriptor for a K-major tile of 128-byte rows written by TMA with the
 // 128-byte swizzle: 8-row groups are 1024 bytes apart (SBO), version 1, layout SWIZZLE_128B.
@@ -216,6 +232,19 @@ __device__ __forceinline__ void umma_commit_cg2_mc(uint64_t* bar, uint16_t cta_m
 __device__ __forceinline__ void named_bar_sync(int id, int n) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
 }
+// the same, returning to every thread whether `ok` held in all of them: a decision to leave a loop is taken together
+__device__ __forceinline__ bool named_bar_all(int id, int n, bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, r;\n\t"
+      "setp.ne.b32 p, %3, 0;\n\t"
+      "bar.red.and.pred r, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, r;\n\t}"
+      : "=r"(all)
+      : "r"(id), "r"(n), "r"((uint32_t)ok)
+      : "memory");
+  return all != 0;
+}
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -238,6 +267,18 @@ constexpr int A_BYTES = BM * BK * 2;
 constexpr int C_SUB = BM * 128;   // one [128 rows x 64 cols] bf16 staging sub-tile
 constexpr int NUM_THREADS = 192;
 constexpr int EPI_THREADS = 128;
+
+// Shared-memory matrix descriptor for an MN-major operand staged as boxes of [64 k-rows x 64 elements (128 bytes)]
+// written by TMA with the 128-byte swizzle (see gemm_bwd_tc.cu).
+constexpr int MN_BOX = 64 * BK * 2;   // one [64 k-rows x 128 B] box
+__device__ __forceinline__ uint64_t make_sdesc_mn128(uint32_t smem_addr) {
+  uint64_t d = (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)(MN_BOX >> 4) << 16;   // leading byte offset: next 64 elements along M/N
+  d |= (uint64_t)(1024 >> 4) << 32;     // stride byte offset: next 8 k-rows
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -264,6 +305,10 @@ struct PipeState {
 // (128 bytes) with the 128-byte swizzle.  Returns 0 on success.
 int make_tmap_bf16_2d(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch_elems,
                       uint32_t box_rows);
+// 3-D f16 tensor [batch, rows, cols], rows `ld` elements and matrices rows * ld elements apart; box = one matrix's
+// [box_rows, 64 cols].  Reads outside a matrix give 0 and stores there are dropped, per matrix.
+int make_tmap_f16_3d(CUtensorMap* out, const void* base, uint64_t batch, uint64_t rows, uint64_t cols, uint64_t ld,
+                     uint32_t box_rows);
 
 }  // namespace tc
 }  // namespace bibo

@@ -655,6 +655,42 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch
     return dx, dweight, dbias
 
 
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of a matrix [m,n] or a stack [..., m, n] (bibo_moe_orthogonalize): with
+    x = update / (|update|_F + eps), ``steps`` times x <- a x + (b G + c G^2) x, G = x x^T.  Returns bf16 [..., m, n],
+    contiguous, whatever the update's type (fp32 or bf16).  ``coefficients`` is one (a, b, c) or one for each step; the
+    polynomials a s + b s^3 + c s^5 must keep singular values of at most 1 below 4.  Rows and matrices may be slices
+    of larger ones; any other order (a transposed view, say) is laid out first."""
+    if not update.is_cuda:
+        raise RuntimeError(f"update is on {update.device}: the bibo_b200 kernels run only on CUDA devices "
+                           "(there is no CPU implementation)")
+    if update.dim() < 2:
+        raise RuntimeError(f"update must be a matrix or a stack of matrices, got shape {tuple(update.shape)}")
+    dt = dtype_code(update.dtype)
+    m, n = update.shape[-2:]
+    u = update.reshape(-1, m, n) if update.numel() else update.reshape(0, m, n)
+    if (n > 1 and u.stride(2) != 1) or (m > 1 and u.stride(1) < n) or (u.shape[0] > 1 and u.stride(0) < (m - 1) * u.stride(1) + n):
+        u = u.contiguous()
+    batch = u.shape[0]
+    steps = int(steps)
+    co = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else list(coefficients)
+    if steps < 1 or len(co) != steps or any(len(c) != 3 for c in co):
+        raise RuntimeError(f"orthogonalize: {steps} steps need one (a, b, c) or {steps} of them")
+    out = torch.empty(update.shape, dtype=torch.bfloat16, device=update.device)
+    if update.numel() == 0:
+        return out
+    lib = _lib.load()
+    ws = torch.empty(int(lib.bibo_moe_orthogonalize_workspace(batch, m, n)), dtype=torch.uint8, device=update.device)
+    flat = (C.c_float * (3 * steps))(*[float(v) for c in co for v in c])
+    p = _lib.ptr
+    _launch("bibo_moe_orthogonalize", update.device, p(u), batch, u.stride(0), m, n, u.stride(1), dt, steps,
+            C.cast(flat, C.c_void_p), float(eps), p(ws), p(out))
+    return out
+
+
 def mlp_forward(x: torch.Tensor, gate_proj: torch.Tensor, up_proj: torch.Tensor, down_proj: torch.Tensor,
                 out: Optional[torch.Tensor] = None, keep: bool = False, residual: Optional[torch.Tensor] = None):
     """Dense SwiGLU MLP ``down(silu(gate(x)) * up(x))`` on flat tokens x [N,H] (bibo_moe_mlp_forward);

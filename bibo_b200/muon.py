@@ -1,0 +1,57 @@
+"""Optimiser for the block's matrices: momentum whose update is orthogonalised on ``bibo_moe_orthogonalize``.
+
+    matrices = [p for p in layer.parameters() if p.requires_grad and p.dim() >= 2]   # gate_proj, gate_up_proj, down_proj
+    opt = bibo_b200.Muon(matrices, lr=0.02)
+
+A stacked parameter [E, m, n] is E matrices, each orthogonalised by itself (``gate_up_proj`` and ``down_proj`` of
+``BiBoFusedExperts``).  Vectors and scalars (``radial_theta``, norm weights) belong to another optimiser and are refused.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import functional as Fn
+
+__all__ = ["Muon"]
+
+
+class Muon(torch.optim.Optimizer):
+    """One step, for a parameter w with gradient g and momentum buffer v (fp32):
+
+        v <- momentum v + g;   u = g + momentum v (nesterov) or v
+        w <- (1 - lr weight_decay) w - lr max(1, m/n)^0.5 orthogonalize(u)
+    """
+
+    def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
+                 steps: int = 5, coefficients=Fn.NEWTON_SCHULZ, eps: float = 1e-7):
+        if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0:
+            raise ValueError(f"Muon: lr={lr}, momentum={momentum}, weight_decay={weight_decay}")
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                                      coefficients=coefficients, eps=eps))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() < 2:
+                    raise ValueError(f"Muon takes matrices and stacks of them, got a parameter of shape {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            momentum = group["momentum"]
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if "momentum_buffer" not in state:
+                    state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+                buf = state["momentum_buffer"]
+                buf.mul_(momentum).add_(p.grad)
+                u = torch.add(p.grad, buf, alpha=momentum) if group["nesterov"] else buf
+                u = Fn.orthogonalize(u.contiguous(), group["steps"], group["coefficients"], group["eps"])
+                if group["weight_decay"]:
+                    p.mul_(1 - group["lr"] * group["weight_decay"])
+                p.add_(u, alpha=-group["lr"] * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5)
+        return loss

@@ -591,6 +591,20 @@ int bibo_moe_dispatch_combine_bwd(const void* dout, int64_t dout_stride, const v
                                   const int32_t* plan, int64_t n_tokens, int hidden, int top_k, int n_experts, int align,
                                   int dtype, void* dys, void* d_topk_w, void* stream);
 
+/* ---- orthogonalised update of stacked matrices -------------------------------------------------------------
+ * For an optimiser that steps along the orthogonal factor of the momentum of the weights whose gradients
+ * bibo_moe_backward produces (the reference's training harness orthogonalises its matrix updates).
+ * u: `batch` matrices [rows, cols], batch_stride and row_stride elements apart.  x_0 = u / (|u|_F + eps), then `steps`
+ * (1..64) times x <- a x + (b G + c G^2) x with G = x x^T (x transposed for tall matrices) and (a, b, c) =
+ * coefficients_host[3 * step ..]; out [batch, rows, cols] is bfloat16 and contiguous.  f16 operands, fp32 accumulation;
+ * the polynomials must keep the singular values below 4 (|b G + c G^2| below 16).  |u|_F^2 is summed in fp32.
+ * workspace: bibo_moe_orthogonalize_workspace bytes, 128-byte aligned (1 GiB at most, more only where one
+ * matrix needs it).  If a bounded wait gives up, the whole result of its group of matrices is NaN.   */
+int64_t bibo_moe_orthogonalize_workspace(int64_t batch, int rows, int cols);
+int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batch_stride, int rows, int cols, int64_t row_stride,
+                           int dtype, int steps, const float* coefficients_host, float eps, void* workspace, void* out,
+                           void* stream);
+
 /* ---- dense SwiGLU MLP -----------------------------------------------------------------------------
  * Replaces BiBoMLP.forward, `down_proj(act_fn(gate_proj(x)) * up_proj(x))` with act = SiLU
  * (src/modeling/ffn/mlp.py:33-34): the shared expert of the MoE layer (src/modeling/ffn/moe.py:120-127,

@@ -139,3 +139,37 @@ def test_shape_stride_and_dtype_checks():
         Fn.combine_backward(rows(4, 32), rows(8, 64), None, plan)
     with pytest.raises(RuntimeError, match="float32 or bfloat16"):
         Fn.combine_forward(rows(8, 64), rows(4, 2, dtype=torch.float16), plan)
+
+
+def test_orthogonalize_refusals_and_workspace():
+    import bibo_b200
+    from bibo_b200 import _lib
+    from bibo_b200 import functional as Fn
+    lib, p = _lib.load(), _dummy()
+    co = (ctypes.c_float * 3)(1.5, -0.5, 0.0)
+    aligned = (p + 127) & ~127
+    call = lambda batch=2, bs=64 * 32, r=64, c=32, rs=32, dt=_lib.F32, steps=1, u=p, ws=aligned, out=p: lib.bibo_moe_orthogonalize(
+        u, batch, bs, r, c, rs, dt, steps, co, 1e-7, ws, out, None)
+    err = lambda: lib.bibo_moe_last_error_string()
+    assert call(dt=3) == -1 and call(steps=0) == -1 and call(steps=65) == -1 and b"steps=65" in err()
+    assert call(rs=31) == -1 and call(bs=64 * 32 - 1) == -1 and b"overlapping" in err()
+    assert call(u=None) == -1 and call(ws=None) == -1 and call(out=None) == -1
+    assert call(ws=aligned + 16) == -2 and call(r=-1) == -1
+    assert call(batch=0) == 0 and call(r=0) == 0
+    size = lib.bibo_moe_orthogonalize_workspace
+    assert size(0, 5, 5) == 0 and size(64, 1024, 2048) == size(64, 2048, 1024) <= 1 << 30
+    assert size(10000, 1024, 2048) <= 1 << 30 and size(1, 20000, 20000) > 1 << 30
+    fake = lambda *s, **k: _fake(torch.zeros(*s, **k))
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        Fn.orthogonalize(torch.zeros(4, 4))
+    with pytest.raises(RuntimeError, match="a matrix or a stack"):
+        Fn.orthogonalize(fake(4))
+    with pytest.raises(RuntimeError, match="float32 or bfloat16"):
+        Fn.orthogonalize(fake(4, 4, dtype=torch.float16))
+    for steps, c in ((0, Fn.NEWTON_SCHULZ), (2, [Fn.NEWTON_SCHULZ]), (1, (1.0, 2.0))):
+        with pytest.raises(RuntimeError, match="steps need"):
+            Fn.orthogonalize(fake(4, 4), steps, c)
+    with pytest.raises(ValueError, match="matrices"):
+        bibo_b200.Muon([torch.nn.Parameter(torch.zeros(4))])
+    with pytest.raises(ValueError, match="momentum"):
+        bibo_b200.Muon([torch.nn.Parameter(torch.zeros(4, 4))], momentum=1.0)
