@@ -197,6 +197,14 @@ __device__ __forceinline__ void tma_load_2d_cg2(void* smem_dst, const CUtensorMa
       ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster_addr), "r"(x), "r"(y)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_cg2(void* smem_dst, const CUtensorMap* m, uint32_t bar_cluster_addr, int x, int y,
+                                                int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
 __device__ __forceinline__ void mbar_arrive_cluster_addr(uint32_t bar_cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
@@ -231,19 +239,6 @@ __device__ __forceinline__ void umma_commit_cg2_mc(uint64_t* bar, uint16_t cta_m
 // named barrier among `n` threads (ids 1..15; 0 is __syncthreads)
 __device__ __forceinline__ void named_bar_sync(int id, int n) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");
-}
-// the same, returning to every thread whether `ok` held in all of them: a decision to leave a loop is taken together
-__device__ __forceinline__ bool named_bar_all(int id, int n, bool ok) {
-  uint32_t all;
-  asm volatile(
-      "{\n\t.reg .pred p, r;\n\t"
-      "setp.ne.b32 p, %3, 0;\n\t"
-      "bar.red.and.pred r, %1, %2, p;\n\t"
-      "selp.u32 %0, 1, 0, r;\n\t}"
-      : "=r"(all)
-      : "r"(id), "r"(n), "r"((uint32_t)ok)
-      : "memory");
-  return all != 0;
 }
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");

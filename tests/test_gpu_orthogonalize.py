@@ -1,15 +1,16 @@
 """Newton-Schulz orthogonalisation against the same steps in 64 bits.
 
-Tolerance.  The result is a bf16 rounding (half a step: 2^-8 relative) of a value computed with f16 operands.  f16 rounds
-to nearest with at most 2^-11 relative per element.  Per step x is rounded once, G once and b G + c G^2 once; the first x of a
-bf16 update not at all.  An elementwise relative perturbation d of a matrix moves it by at most d |.|_F in the Frobenius
-norm.  With singular values s <= 1.2 and s the largest slope of the polynomial (a = 3.4445) the error E_k = |x_k - exact|_F
-grows at most as
-    E_{k+1} <= L E_k + d (|x_k|_F |F_k|_2 + |G_k|_F |b| |x_k|_2 + |F_k|_F |x_k|_2 + |x_{k+1}|_F) + 2 |c| |G|_2 d |G|_F |x|_2,
-F = b G + c G^2, L the Lipschitz constant of the matrix polynomial, which the test evaluates as a plus the derivatives of the
-other two terms.  That worst case adds all roundings with one sign; independent ones add as squares, so the test evaluates the
-recursion in the root-mean-square sense instead: d = 2^-11 / sqrt(3), terms added in squares, L = the largest |p'(s)| over the
-singular values present (the perturbation is spread over the singular directions).  A factor 4 covers the distribution's tail."""
+Tolerance.  The result is a bf16 rounding (half a step: 2^-8 relative) of a value computed with f16 operands.  f16 rounds to
+nearest with at most 2^-11 relative per element; with d = 2^-11 / sqrt(3) the root mean square of it, rounding a matrix M
+moves it by d |M|_F in the Frobenius norm.  With F = b G + c G^2, single roundings of independent sign (so the terms add as
+squares) and |.| the spectral norm, a step x' = a x + F x has
+    dG = d |G|_F,   dF = d |F|_F + (|b| + 2 |c| |G|) dG,   dx' = L dx + |x| dF + d |x'|_F
+where L is the slope of a s + b s^3 + c s^5 over the singular values present (at least a).  Where two steps are joined
+(x'' = a1 a2 x + R x; no x' is rounded, x'' is kept in two halves):
+    dT = d |T|_F + 2 (a1 + |F1|) dF1,   dG' = d |G'|_F + |T| dG + |G| dT,   dF2 = d |F2|_F + (|b2| + 2 |c2| |G'|) dG',
+    dR = d |R|_F + (a1 + |F1|) dF2 + (a2 + |F2|) dF1,   dx'' = L1 L2 dx + |x| dR
+dx starts at 0: a bf16 update is held exactly, an fp32 one in two halves (2^-22) in the terms "a x", while the rounding of the
+other factor, d |x|_F, enters through |F| or |R|, which is added.  A factor 4 covers the tail of the distribution."""
 import math
 
 import pytest
@@ -28,18 +29,42 @@ def _steps64(u, steps, coefficients, eps=1e-7):
     x = x.mT if tall else x
     x = x / (x.flatten(-2).norm(dim=-1)[..., None, None] + eps)
     fro = lambda a: a.flatten(-2).norm(dim=-1)
-    err2 = (D * fro(x)) ** 2 if u.dtype == torch.float32 else torch.zeros_like(fro(x))
-    for k in range(steps):
-        a, b, c = coefficients[k] if hasattr(coefficients[0], "__len__") else coefficients
+    top = lambda a: torch.linalg.matrix_norm(a.cpu(), 2).to(DEV)
+    co = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else coefficients
+    one = torch.eye(x.shape[-2], dtype=x.dtype, device=DEV)
+    err2 = torch.zeros_like(fro(x))
+    first = (D * fro(x)) ** 2 if u.dtype == torch.float32 else 0 * err2       # the rounded operand of the first product
+
+    def polynomial(g, c):
+        f = c[1] * g + c[2] * (g @ g)
+        s = torch.linalg.eigvalsh(g.cpu()).to(DEV).clamp_min(0)
+        return f, (c[0] + 3 * c[1] * s + 5 * c[2] * s ** 2).abs().amax(-1).clamp_min(abs(c[0]))
+
+    k = 0
+    if steps >= 3:
+        (a1, b1, c1), (a2, b2, c2) = co[:2]
         g = x @ x.mT
-        f = b * g + c * (g @ g)
-        new = a * x + f @ x
-        s = torch.linalg.svdvals(g.cpu()).to(DEV).clamp_min(0).sqrt()
-        slope = (a + 3 * b * s ** 2 + 5 * c * s ** 4).abs().amax(-1).clamp_min(abs(a))
-        top = s.amax(-1)
-        df2 = (D * fro(f)) ** 2 + (D * abs(b) * fro(g)) ** 2 + (2 * abs(c) * top ** 2 * D * fro(g)) ** 2
-        err2 = slope ** 2 * err2 + df2 * top ** 2 + (D * fro(new)) ** 2
-        x = new
+        f1, l1 = polynomial(g, co[0])
+        t = f1 @ f1 + 2 * a1 * f1
+        g2 = a1 * a1 * g + t @ g
+        f2, l2 = polynomial(g2, co[1])
+        r = f2 @ f1 + a1 * f2 + a2 * f1
+        new = (a2 * one + f2) @ ((a1 * one + f1) @ x)
+        dg = (D * fro(g)) ** 2
+        df1 = (D * fro(f1)) ** 2 + (abs(b1) + 2 * abs(c1) * top(g)) ** 2 * dg
+        dt = (D * fro(t)) ** 2 + 4 * (a1 + top(f1)) ** 2 * df1
+        dg2 = (D * fro(g2)) ** 2 + top(t) ** 2 * dg + top(g) ** 2 * dt
+        df2 = (D * fro(f2)) ** 2 + (abs(b2) + 2 * abs(c2) * top(g2)) ** 2 * dg2
+        dr = (D * fro(r)) ** 2 + (a1 + top(f1)) ** 2 * df2 + (a2 + top(f2)) ** 2 * df1
+        err2 = top(x) ** 2 * dr + top(r) ** 2 * first
+        first, x, k = (D * fro(new)) ** 2, new, 2
+    for k in range(k, steps):
+        g = x @ x.mT
+        f, slope = polynomial(g, co[k])
+        new = co[k][0] * x + f @ x
+        df = (D * fro(f)) ** 2 + (abs(co[k][1]) + 2 * abs(co[k][2]) * top(g)) ** 2 * (D * fro(g)) ** 2
+        err2 = slope ** 2 * err2 + top(x) ** 2 * df + top(f) ** 2 * first + (D * fro(new)) ** 2
+        first, x = 0 * err2, new
     return (x.mT if tall else x), err2.sqrt()
 
 

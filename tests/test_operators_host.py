@@ -157,8 +157,8 @@ def test_orthogonalize_refusals_and_workspace():
     assert call(ws=aligned + 16) == -2 and call(r=-1) == -1
     assert call(batch=0) == 0 and call(r=0) == 0
     size = lib.bibo_moe_orthogonalize_workspace
-    assert size(0, 5, 5) == 0 and size(64, 1024, 2048) == size(64, 2048, 1024) <= 1 << 30
-    assert size(10000, 1024, 2048) <= 1 << 30 and size(1, 20000, 20000) > 1 << 30
+    assert size(0, 5, 5) == 0 and size(64, 1024, 2048) == size(64, 2048, 1024) <= 1 << 31
+    assert size(10000, 1024, 2048) <= 1 << 31 and size(1, 20000, 20000) > 1 << 31
     fake = lambda *s, **k: _fake(torch.zeros(*s, **k))
     with pytest.raises(RuntimeError, match="no CPU implementation"):
         Fn.orthogonalize(torch.zeros(4, 4))
