@@ -192,36 +192,41 @@ __device__ __forceinline__ void zero_empty_rows(const int32_t* __restrict__ row_
   }
 }
 
-// warps [0, N): a token's row is read once and written to its (up to k) rows; warps behind them zero empty rows
+// Work items: (token, part of the row) for a warp each, then blocks whose warps zero the rows without a slot.
+// A part is `part` accesses of 32 lanes; few tokens are cut into many parts so that the machine is not left to a few warps.
+
+// a token's row is read once and written to its (up to k) rows; eight loads of a lane are in flight before the first store
 template <int VB>
 __global__ void __launch_bounds__(DW * 32)
 dispatch_kernel(const uint8_t* __restrict__ x, int64_t x_stride_bytes, const int32_t* __restrict__ slot_row,
-                const int32_t* __restrict__ row_slot, int64_t n_tokens, int top_k, int64_t rows, int row_bytes,
+                const int32_t* __restrict__ row_slot, int64_t n_tokens, int top_k, int64_t rows, int chunks, int parts, int part,
                 uint8_t* __restrict__ xs) {
   using V = typename RowVec<VB>::type;
   const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * DW + (threadIdx.x >> 5);
-  const int chunks = row_bytes / VB;
   V* dst = reinterpret_cast<V*>(xs);
-  if (w >= n_tokens) {
-    zero_empty_rows<VB>(row_slot, (w - n_tokens) * DZ_ROWS, rows, chunks, dst, lane);
+  const int64_t items = n_tokens * parts;
+  if (w >= items) {
+    zero_empty_rows<VB>(row_slot, (w - items) * DZ_ROWS, rows, chunks, dst, lane);
     return;
   }
-  const int mine = lane < top_k ? slot_row[w * top_k + lane] : -1;
-  if (!__any_sync(0xffffffffu, mine >= 0)) return;
-  const V* src = reinterpret_cast<const V*>(x + w * x_stride_bytes);
-  for (int c0 = lane; c0 - lane < chunks; c0 += 256) {
+  const int64_t t = parts == 1 ? w : w / parts;
+  const int mine = lane < top_k ? slot_row[t * top_k + lane] : -1;
+  const V* src = reinterpret_cast<const V*>(x + t * x_stride_bytes);
+  const int c_lo = parts == 1 ? 0 : (int)(w % parts) * part * 32, c_hi = min(chunks, c_lo + part * 32);
+  const unsigned filled = __ballot_sync(0xffffffffu, mine >= 0);
+  if (!filled) return;
+  for (int c0 = c_lo + lane; c0 - lane < c_hi; c0 += 256) {
     V v[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (c0 + u * 32 < chunks) v[u] = src[c0 + u * 32];
-    for (int j = 0; j < top_k; ++j) {
-      const int r = __shfl_sync(0xffffffffu, mine, j);
-      if (r < 0) continue;
+      if (c0 + u * 32 < c_hi) v[u] = src[c0 + u * 32];
+    for (unsigned todo = filled; todo; todo &= todo - 1) {
+      const int r = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
       V* d = dst + (int64_t)r * chunks;
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (c0 + u * 32 < chunks) d[c0 + u * 32] = v[u];
+        if (c0 + u * 32 < c_hi) d[c0 + u * 32] = v[u];
     }
   }
 }
@@ -231,83 +236,136 @@ __device__ __forceinline__ float load_weight(const void* w, int is_bf16, int64_t
   return is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]) : static_cast<const float*>(w)[i];
 }
 
-// out[t] = sum_j w[t,j] * ys[slot_row[t,j]] (w == nullptr: 1), a warp per token, slots in order
-template <typename T, int VB>
+// out[t] = sum_j w[t,j] * ys[slot_row[t,j]] (weight == nullptr: 1), slots in order.  All K loads of U accesses are issued before
+// the first is used; K slots a round, and further rounds for k > K.
+template <typename T, int VB, int K, int U>
 __global__ void __launch_bounds__(DW * 32)
 dispatch_combine_kernel(const T* __restrict__ ys, const void* __restrict__ weight, int w_bf16,
-                        const int32_t* __restrict__ slot_row, int64_t n_tokens, int top_k, int hidden, T* __restrict__ out) {
+                        const int32_t* __restrict__ slot_row, int64_t n_tokens, int top_k, int chunks, int parts, int part,
+                        T* __restrict__ out) {
   using V = typename RowVec<VB>::type;
   using X = RowElems<T, VB>;
   const int lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * DW + (threadIdx.x >> 5);
+  const int64_t wi = (int64_t)blockIdx.x * DW + (threadIdx.x >> 5);
+  const int64_t t = parts == 1 ? wi : wi / parts;
   if (t >= n_tokens) return;
-  const int chunks = hidden / X::N;
   const int mine = lane < top_k ? slot_row[t * top_k + lane] : -1;
   const float my_w = mine < 0 ? 0.f : weight == nullptr ? 1.f : load_weight(weight, w_bf16, t * top_k + lane);
   const V* src = reinterpret_cast<const V*>(ys);
   V* dst = reinterpret_cast<V*>(out) + t * chunks;
-  for (int c0 = 0; c0 < chunks; c0 += 32) {
-    const int c = c0 + lane;
-    float acc[X::N];
+  const int c_lo = parts == 1 ? 0 : (int)(wi % parts) * part * 32, c_hi = min(chunks, c_lo + part * 32);
+  for (int c0 = c_lo + lane; c0 - lane < c_hi; c0 += 32 * U) {
+    float acc[U][X::N];
 #pragma unroll
-    for (int i = 0; i < X::N; ++i) acc[i] = 0.f;
-    for (int j = 0; j < top_k; ++j) {
-      const int r = __shfl_sync(0xffffffffu, mine, j);
-      const float w = __shfl_sync(0xffffffffu, my_w, j);
-      if (r < 0 || c >= chunks) continue;
-      float f[X::N];
-      X::unpack(src[(int64_t)r * chunks + c], f);
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < X::N; ++i) acc[i] = fmaf(f[i], w, acc[i]);
+      for (int i = 0; i < X::N; ++i) acc[u][i] = 0.f;
+    for (int j0 = 0; j0 < top_k; j0 += K) {
+      V v[U][K];
+      int r[K];
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        r[j] = j0 + j < 32 ? __shfl_sync(0xffffffffu, mine, j0 + j) : -1;       // lanes beyond k hold -1
+        const V* row = src + (int64_t)r[j] * chunks;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (r[j] >= 0 && c0 + u * 32 < c_hi) v[u][j] = __ldcs(row + c0 + u * 32);
+      }
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        const float w = __shfl_sync(0xffffffffu, my_w, (j0 + j) & 31);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (r[j] >= 0 && c0 + u * 32 < c_hi) {
+            float f[X::N];
+            X::unpack(v[u][j], f);
+#pragma unroll
+            for (int i = 0; i < X::N; ++i) acc[u][i] = fmaf(f[i], w, acc[u][i]);
+          }
+      }
     }
-    if (c < chunks) dst[c] = X::pack(acc);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * 32 < c_hi) dst[c0 + u * 32] = X::pack(acc[u]);
   }
 }
 
-// warps [0, N): dys rows and dw of a token's slots; warps behind them zero empty rows of dys
-template <typename T, int VB>
+// dys rows and dw of a token's slots, WPT warps per token (1, or all DW for few tokens) that share its columns; blocks behind
+// the tokens' zero the rows of dys without a slot
+template <typename T, int VB, int K>
 __global__ void __launch_bounds__(DW * 32)
 dispatch_combine_bwd_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __restrict__ ys,
                             const void* __restrict__ weight, int w_bf16, const int32_t* __restrict__ slot_row,
-                            const int32_t* __restrict__ row_slot, int64_t n_tokens, int top_k, int64_t rows, int hidden,
-                            T* __restrict__ dys, void* __restrict__ dweight) {
+                            const int32_t* __restrict__ row_slot, int64_t n_tokens, int top_k, int64_t rows, int chunks, int wpt,
+                            int64_t token_blocks, T* __restrict__ dys, void* __restrict__ dweight) {
   using V = typename RowVec<VB>::type;
   using X = RowElems<T, VB>;
-  const int lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * DW + (threadIdx.x >> 5);
-  const int chunks = hidden / X::N;
+  __shared__ float red[DW][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   V* dst = reinterpret_cast<V*>(dys);
-  if (t >= n_tokens) {
-    zero_empty_rows<VB>(row_slot, (t - n_tokens) * DZ_ROWS, rows, chunks, dst, lane);
+  if ((int64_t)blockIdx.x >= token_blocks) {
+    zero_empty_rows<VB>(row_slot, (((int64_t)blockIdx.x - token_blocks) * DW + warp) * DZ_ROWS, rows, chunks, dst, lane);
     return;
   }
+  const int64_t t = wpt == 1 ? (int64_t)blockIdx.x * DW + warp : blockIdx.x;
+  const bool in = t < n_tokens;
   const V* g = reinterpret_cast<const V*>(dout + t * dout_stride);
   const V* src = reinterpret_cast<const V*>(ys);
-  const int mine = lane < top_k ? slot_row[t * top_k + lane] : -1;
+  const int mine = in && lane < top_k ? slot_row[t * top_k + lane] : -1;
   const float my_w = mine < 0 ? 0.f : weight == nullptr ? 1.f : load_weight(weight, w_bf16, t * top_k + lane);
+  const bool want = dweight != nullptr;
   float my_dw = 0.f;
-  for (int j = 0; j < top_k; ++j) {
-    const int r = __shfl_sync(0xffffffffu, mine, j);
-    const float w = __shfl_sync(0xffffffffu, my_w, j);
-    if (r < 0) continue;
-    float dot = 0.f;
-    for (int c = lane; c < chunks; c += 32) {
-      float gf[X::N], yf[X::N];
-      X::unpack(g[c], gf);
-      if (dweight != nullptr) {
-        X::unpack(src[(int64_t)r * chunks + c], yf);
+  if (__any_sync(0xffffffffu, mine >= 0)) {
+    for (int j0 = 0; j0 < top_k; j0 += K) {
+      float dot[K], w[K];
+      int r[K];
 #pragma unroll
-        for (int i = 0; i < X::N; ++i) dot = fmaf(gf[i], yf[i], dot);
+      for (int j = 0; j < K; ++j) {
+        dot[j] = 0.f;
+        r[j] = j0 + j < 32 ? __shfl_sync(0xffffffffu, mine, j0 + j) : -1;
+        w[j] = __shfl_sync(0xffffffffu, my_w, (j0 + j) & 31);
       }
+      for (int c = (wpt == 1 ? 0 : warp * 32) + lane; c < chunks; c += 32 * wpt) {
+        V gv = g[c], v[K];
 #pragma unroll
-      for (int i = 0; i < X::N; ++i) gf[i] *= w;
-      dst[(int64_t)r * chunks + c] = X::pack(gf);
+        for (int j = 0; j < K; ++j)
+          if (want && r[j] >= 0) v[j] = __ldcs(src + (int64_t)r[j] * chunks + c);
+        float gf[X::N];
+        X::unpack(gv, gf);
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+          if (r[j] >= 0) {
+            float f[X::N];
+            if (want) {
+              X::unpack(v[j], f);
+#pragma unroll
+              for (int i = 0; i < X::N; ++i) dot[j] = fmaf(gf[i], f[i], dot[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < X::N; ++i) f[i] = gf[i] * w[j];
+            dst[(int64_t)r[j] * chunks + c] = X::pack(f);
+          }
+      }
+      if (want) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+          if (lane == j0 + j) my_dw = dot[j];
+        }
+      }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if (lane == j) my_dw = dot;
   }
-  if (dweight != nullptr && lane < top_k) {
+  if (!want) return;
+  if (wpt > 1) {
+    red[warp][lane] = my_dw;
+    __syncthreads();
+    if (warp != 0) return;
+    my_dw = 0.f;
+#pragma unroll
+    for (int i = 0; i < DW; ++i) my_dw += red[i][lane];
+  }
+  if (in && lane < top_k) {
     if (w_bf16) static_cast<__nv_bfloat16*>(dweight)[t * top_k + lane] = __float2bfloat16_rn(my_dw);
     else static_cast<float*>(dweight)[t * top_k + lane] = my_dw;
   }
@@ -329,6 +387,14 @@ static int dispatch_check(const char* what, int64_t n_tokens, int hidden, int n_
   return BIBO_OK;
 }
 static unsigned dispatch_grid(int64_t warps) { return (unsigned)((warps + DW - 1) / DW); }
+// parts a row is cut into, and their size in accesses of a warp: enough warps for every SM to have 16, where the row allows it
+static int row_parts(int64_t n_tokens, int chunks, int* part) {
+  const int steps = (chunks + 31) / 32;
+  const int64_t want = (16 * (int64_t)sm_count() + n_tokens - 1) / n_tokens;
+  const int parts = want < steps ? (int)want : steps;
+  *part = (steps + parts - 1) / parts;
+  return (steps + *part - 1) / *part;
+}
 
 template <typename I>
 static int plan_launch(const void* idx, int64_t slots, int E, int align, int32_t* plan, cudaStream_t st) {
@@ -399,13 +465,17 @@ extern "C" int bibo_moe_dispatch_fwd(const void* x, int64_t x_stride, const int3
   const int32_t* row_slot = plan + dp_off_row_slot(n_experts, slots);
   const int row_bytes = hidden * size;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const unsigned grid = dispatch_grid(n_tokens + (rows + DZ_ROWS - 1) / DZ_ROWS);
+  const int vb = row_vec_bytes(row_bytes, n_tokens > 1 ? x_stride * size : 0, x, xs, nullptr);
+  const int chunks = row_bytes / vb;
+  int part;
+  const int parts = row_parts(n_tokens, chunks, &part);
+  const unsigned grid = dispatch_grid(n_tokens * parts + (rows + DZ_ROWS - 1) / DZ_ROWS);
 #define BIBO_DISPATCH_CASE(VB)                                                                                              \
   case VB:                                                                                                                  \
     dispatch_kernel<VB><<<grid, DW * 32, 0, st>>>(static_cast<const uint8_t*>(x), x_stride * size, slot_row, row_slot,      \
-                                                  n_tokens, top_k, rows, row_bytes, static_cast<uint8_t*>(xs));             \
+                                                  n_tokens, top_k, rows, chunks, parts, part, static_cast<uint8_t*>(xs));   \
     break;
-  switch (row_vec_bytes(row_bytes, n_tokens > 1 ? x_stride * size : 0, x, xs, nullptr)) {
+  switch (vb) {
     BIBO_DISPATCH_CASE(16) BIBO_DISPATCH_CASE(8) BIBO_DISPATCH_CASE(4) BIBO_DISPATCH_CASE(2)
   }
 #undef BIBO_DISPATCH_CASE
@@ -413,16 +483,30 @@ extern "C" int bibo_moe_dispatch_fwd(const void* x, int64_t x_stride, const int3
   return BIBO_OK;
 }
 
+template <typename T, int VB>
+static void combine_v(const void* ys, const void* weight, int w_bf16, const int32_t* slot_row, int64_t n_tokens, int top_k,
+                      int hidden, void* out, cudaStream_t st) {
+  const int chunks = hidden / RowElems<T, VB>::N;
+  int part;
+  const int parts = row_parts(n_tokens, chunks, &part);
+  const unsigned grid = dispatch_grid(n_tokens * parts);
+#define BIBO_COMBINE(K, U)                                                                                                  \
+  dispatch_combine_kernel<T, VB, K, U><<<grid, DW * 32, 0, st>>>(static_cast<const T*>(ys), weight, w_bf16, slot_row, n_tokens, \
+                                                                 top_k, chunks, parts, part, static_cast<T*>(out))
+  if (top_k == 1) BIBO_COMBINE(1, 4);
+  else if (top_k == 2) BIBO_COMBINE(2, 4);
+  else if (top_k <= 4) BIBO_COMBINE(4, 2);
+  else if (top_k <= 6) BIBO_COMBINE(6, 2);
+  else BIBO_COMBINE(8, 2);
+#undef BIBO_COMBINE
+}
 template <typename T>
 static int combine_t(const void* ys, const void* weight, int w_bf16, const int32_t* slot_row, int64_t n_tokens, int top_k,
                      int hidden, void* out, cudaStream_t st) {
-  const unsigned grid = dispatch_grid(n_tokens);
   const int vb = row_vec_bytes((int64_t)hidden * sizeof(T), 0, ys, out, nullptr);
 #define BIBO_DISPATCH_CASE(VB)                                                                                               \
   if constexpr (VB >= (int)sizeof(T))                                                                                        \
-    if (vb == VB)                                                                                                            \
-      dispatch_combine_kernel<T, VB><<<grid, DW * 32, 0, st>>>(static_cast<const T*>(ys), weight, w_bf16, slot_row, n_tokens, \
-                                                               top_k, hidden, static_cast<T*>(out));
+    if (vb == VB) combine_v<T, VB>(ys, weight, w_bf16, slot_row, n_tokens, top_k, hidden, out, st);
   BIBO_DISPATCH_CASE(16) BIBO_DISPATCH_CASE(8) BIBO_DISPATCH_CASE(4) BIBO_DISPATCH_CASE(2)
 #undef BIBO_DISPATCH_CASE
   BIBO_CHECK_LAUNCH("dispatch_combine_kernel");
@@ -444,18 +528,36 @@ extern "C" int bibo_moe_dispatch_combine_fwd(const void* ys, const void* topk_w,
                            : combine_t<__nv_bfloat16>(ys, topk_w, wb, slot_row, n_tokens, top_k, hidden, out, st);
 }
 
+template <typename T, int VB>
+static void combine_bwd_v(const void* dout, int64_t dout_stride, const void* ys, const void* weight, int w_bf16,
+                          const int32_t* slot_row, const int32_t* row_slot, int64_t n_tokens, int top_k, int64_t rows, int hidden,
+                          void* dys, void* dweight, cudaStream_t st) {
+  const int chunks = hidden / RowElems<T, VB>::N;
+  const int wpt = n_tokens < 4 * (int64_t)sm_count() ? DW : 1;      // a block per token where warps per token would be few
+  const int64_t token_blocks = wpt == 1 ? (n_tokens + DW - 1) / DW : n_tokens;
+  const unsigned grid = (unsigned)token_blocks + dispatch_grid((rows + DZ_ROWS - 1) / DZ_ROWS);
+#define BIBO_COMBINE(K)                                                                                                      \
+  dispatch_combine_bwd_kernel<T, VB, K><<<grid, DW * 32, 0, st>>>(static_cast<const T*>(dout), dout_stride,                  \
+                                                                  static_cast<const T*>(ys), weight, w_bf16, slot_row,       \
+                                                                  row_slot, n_tokens, top_k, rows, chunks, wpt, token_blocks, \
+                                                                  static_cast<T*>(dys), dweight)
+  if (top_k == 1) BIBO_COMBINE(1);
+  else if (top_k == 2) BIBO_COMBINE(2);
+  else if (top_k <= 4) BIBO_COMBINE(4);
+  else if (top_k <= 6) BIBO_COMBINE(6);
+  else BIBO_COMBINE(8);
+#undef BIBO_COMBINE
+}
 template <typename T>
 static int combine_bwd_t(const void* dout, int64_t dout_stride, const void* ys, const void* weight, int w_bf16,
                          const int32_t* slot_row, const int32_t* row_slot, int64_t n_tokens, int top_k, int64_t rows, int hidden,
                          void* dys, void* dweight, cudaStream_t st) {
-  const unsigned grid = dispatch_grid(n_tokens + (rows + DZ_ROWS - 1) / DZ_ROWS);
   const int vb = row_vec_bytes((int64_t)hidden * sizeof(T), n_tokens > 1 ? dout_stride * (int64_t)sizeof(T) : 0, dout, ys, dys);
-#define BIBO_DISPATCH_CASE(VB)                                                                                          \
-  if constexpr (VB >= (int)sizeof(T))                                                                                   \
-    if (vb == VB)                                                                                                       \
-      dispatch_combine_bwd_kernel<T, VB><<<grid, DW * 32, 0, st>>>(                                                     \
-          static_cast<const T*>(dout), dout_stride, static_cast<const T*>(ys), weight, w_bf16, slot_row, row_slot,      \
-          n_tokens, top_k, rows, hidden, static_cast<T*>(dys), dweight);
+#define BIBO_DISPATCH_CASE(VB)                                                                                              \
+  if constexpr (VB >= (int)sizeof(T))                                                                                       \
+    if (vb == VB)                                                                                                           \
+      combine_bwd_v<T, VB>(dout, dout_stride, ys, weight, w_bf16, slot_row, row_slot, n_tokens, top_k, rows, hidden, dys,   \
+                           dweight, st);
   BIBO_DISPATCH_CASE(16) BIBO_DISPATCH_CASE(8) BIBO_DISPATCH_CASE(4) BIBO_DISPATCH_CASE(2)
 #undef BIBO_DISPATCH_CASE
   BIBO_CHECK_LAUNCH("dispatch_combine_bwd_kernel");

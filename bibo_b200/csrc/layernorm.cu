@@ -8,6 +8,263 @@
 
 namespace bibo {
 
+// ---- rows held in registers ------------------------------------------------------------------------------------
+// VE elements per access: 16 bytes where rows, strides and pointers allow it, else 4 (bf16 pairs) or one element.
+template <typename T, int VE> struct LnVec;
+template <> struct LnVec<float, 4> {
+  using V = uint4;
+  static __device__ __forceinline__ void unpack(const V& v, float* f) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ V pack(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
+template <> struct LnVec<float, 1> {
+  using V = float;
+  static __device__ __forceinline__ void unpack(const V& v, float* f) { f[0] = v; }
+  static __device__ __forceinline__ V pack(const float* f) { return f[0]; }
+};
+template <> struct LnVec<__nv_bfloat16, 8> {
+  using V = uint4;
+  static __device__ __forceinline__ void unpack(const V& v, float* f) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(u[i] << 16); f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+  }
+  static __device__ __forceinline__ V pack(const float* f) {
+    V v;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    return v;
+  }
+};
+template <> struct LnVec<__nv_bfloat16, 2> {
+  using V = uint32_t;
+  static __device__ __forceinline__ void unpack(const V& v, float* f) {
+    f[0] = __uint_as_float(v << 16); f[1] = __uint_as_float(v & 0xffff0000u);
+  }
+  static __device__ __forceinline__ V pack(const float* f) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(f[0], f[1]);
+    return *reinterpret_cast<const V*>(&h);
+  }
+};
+template <> struct LnVec<__nv_bfloat16, 1> {
+  using V = __nv_bfloat16;
+  static __device__ __forceinline__ void unpack(const V& v, float* f) { f[0] = __bfloat162float(v); }
+  static __device__ __forceinline__ V pack(const float* f) { return __float2bfloat16_rn(f[0]); }
+};
+// VE parameters [c * VE, (c + 1) * VE) as fp32
+template <typename W, int VE> __device__ __forceinline__ void ln_param(const W* __restrict__ w, int c, float* f) {
+  if constexpr (VE == 8 && sizeof(W) == 4) {
+    LnVec<float, 4>::unpack(__ldg(reinterpret_cast<const uint4*>(w) + 2 * c), f);
+    LnVec<float, 4>::unpack(__ldg(reinterpret_cast<const uint4*>(w) + 2 * c + 1), f + 4);
+  } else if constexpr (VE == 2 && sizeof(W) == 4) {
+    const float2 v = __ldg(reinterpret_cast<const float2*>(w) + c);
+    f[0] = v.x; f[1] = v.y;
+  } else {
+    using X = LnVec<W, VE>;
+    X::unpack(reinterpret_cast<const typename X::V*>(w)[c], f);
+  }
+}
+
+// sum over the G threads of a row: a warp, or the block
+template <int G> __device__ __forceinline__ float ln_row_sum(float a, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if (G > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    __syncthreads();
+    a = 0.f;
+#pragma unroll
+    for (int w = 0; w < G / 32; ++w) a += red[w];
+  }
+  return a;
+}
+
+// Forward: G threads per row (32: eight rows a block), CH accesses per thread; one read and one write of a row.
+template <typename T, typename W, int VE, int G, int CH>
+__global__ void __launch_bounds__(G > 32 ? G : 256)
+layernorm_kernel(const T* __restrict__ x, int64_t x_stride, const W* __restrict__ weight, const W* __restrict__ bias, float eps,
+                 int64_t n_rows, int hidden, T* __restrict__ out, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+  using X = LnVec<T, VE>;
+  using V = typename X::V;
+  __shared__ float red[2][G > 32 ? G / 32 : 1];
+  const int lane = G > 32 ? threadIdx.x : threadIdx.x & 31;
+  const int64_t row = G > 32 ? blockIdx.x : (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (G == 32 && row >= n_rows) return;
+  const V* src = reinterpret_cast<const V*>(x + row * x_stride);
+  V* dst = reinterpret_cast<V*>(out + row * hidden);
+  const int vecs = hidden / VE;
+  V v[CH];
+  float s = 0.f;
+#pragma unroll
+  for (int q = 0; q < CH; ++q)
+    if (q * G + lane < vecs) v[q] = __ldcs(src + q * G + lane);
+#pragma unroll
+  for (int q = 0; q < CH; ++q)
+    if (q * G + lane < vecs) {
+      float f[VE];
+      X::unpack(v[q], f);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) s += f[i];
+    }
+  const float inv = 1.f / (float)hidden;
+  const float mean = ln_row_sum<G>(s, red[0]) * inv;
+  s = 0.f;
+#pragma unroll
+  for (int q = 0; q < CH; ++q)
+    if (q * G + lane < vecs) {
+      float f[VE];
+      X::unpack(v[q], f);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) { const float d = f[i] - mean; s = fmaf(d, d, s); }
+    }
+  const float rstd = rsqrtf(fmaf(ln_row_sum<G>(s, red[1]), inv, eps));
+  if (lane == 0 && mean_out != nullptr) { mean_out[row] = mean; rstd_out[row] = rstd; }
+#pragma unroll
+  for (int q = 0; q < CH; ++q)
+    if (q * G + lane < vecs) {
+      const int c = q * G + lane;
+      float f[VE], w[VE], b[VE];
+      X::unpack(v[q], f);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) { w[i] = 1.f; b[i] = 0.f; }
+      if (weight != nullptr) ln_param<W, VE>(weight, c, w);
+      if (bias != nullptr) ln_param<W, VE>(bias, c, b);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) f[i] = fmaf((f[i] - mean) * rstd, w[i], b[i]);
+      dst[c] = X::pack(f);
+    }
+}
+
+// Backward: a block of NT threads walks over groups of R rows; a thread owns CH x VE columns, whose weight and bias gradients it
+// carries in registers over all its rows.  The 2 R row sums of a group cross the block at once: one barrier per R rows.
+// Each block leaves one row of partial sums; layernorm_dparam_kernel adds them in a fixed order.
+template <typename T, typename W, int VE, int NT, int CH, int R>
+__global__ void __launch_bounds__(NT)
+layernorm_bwd_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ dy, int64_t dy_stride,
+                     const W* __restrict__ weight, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+                     int64_t n_rows, int hidden, T* __restrict__ dx, float* __restrict__ partial) {
+  using X = LnVec<T, VE>;
+  using V = typename X::V;
+  constexpr int WARPS = NT / 32;
+  __shared__ float red[2][WARPS][2 * R];
+  const int tid = threadIdx.x;
+  const int vecs = hidden / VE;
+  const float inv = 1.f / (float)hidden;
+  float dw[CH][VE], db[CH][VE];
+#pragma unroll
+  for (int q = 0; q < CH; ++q)
+#pragma unroll
+    for (int i = 0; i < VE; ++i) dw[q][i] = db[q][i] = 0.f;
+  int buf = 0;
+  for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < n_rows; row0 += (int64_t)gridDim.x * R, buf ^= 1) {
+    V xv[R][CH], gv[R][CH];
+    float mean[R], rstd[R], s[2 * R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const bool in = row0 + r < n_rows;
+      const V* xs = reinterpret_cast<const V*>(x + (row0 + r) * x_stride);
+      const V* gs = reinterpret_cast<const V*>(dy + (row0 + r) * dy_stride);
+      mean[r] = in ? mean_in[row0 + r] : 0.f;
+      rstd[r] = in ? rstd_in[row0 + r] : 0.f;
+#pragma unroll
+      for (int q = 0; q < CH; ++q) {
+        const int c = q * NT + tid;
+        if (in && c < vecs) { xv[r][q] = __ldcs(xs + c); gv[r][q] = __ldcs(gs + c); }
+        else { xv[r][q] = V{}; gv[r][q] = V{}; }          // adds nothing anywhere
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float a = 0.f, b = 0.f;
+#pragma unroll
+      for (int q = 0; q < CH; ++q) {
+        float f[VE], g[VE], w[VE];
+        X::unpack(xv[r][q], f);
+        X::unpack(gv[r][q], g);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) w[i] = 1.f;
+        if (weight != nullptr && q * NT + tid < vecs) ln_param<W, VE>(weight, q * NT + tid, w);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          const float z = (f[i] - mean[r]) * rstd[r], gw = g[i] * w[i];
+          a += gw;
+          b = fmaf(gw, z, b);
+          dw[q][i] = fmaf(g[i], z, dw[q][i]);
+          db[q][i] += g[i];
+        }
+      }
+      s[2 * r] = a;
+      s[2 * r + 1] = b;
+    }
+#pragma unroll
+    for (int k = 0; k < 2 * R; ++k)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
+    if (WARPS > 1) {
+      if ((tid & 31) == 0)
+#pragma unroll
+        for (int k = 0; k < 2 * R; ++k) red[buf][tid >> 5][k] = s[k];
+      __syncthreads();                     // the other buffer's readers are a full group behind
+#pragma unroll
+      for (int k = 0; k < 2 * R; ++k) s[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w)
+#pragma unroll
+        for (int k = 0; k < 2 * R; ++k) s[k] += red[buf][w][k];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (row0 + r >= n_rows) continue;
+      V* ds = reinterpret_cast<V*>(dx + (row0 + r) * hidden);
+      const float m0 = s[2 * r] * inv, m1 = s[2 * r + 1] * inv;
+#pragma unroll
+      for (int q = 0; q < CH; ++q) {
+        const int c = q * NT + tid;
+        if (c >= vecs) continue;
+        float f[VE], g[VE], w[VE];
+        X::unpack(xv[r][q], f);
+        X::unpack(gv[r][q], g);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) w[i] = 1.f;
+        if (weight != nullptr) ln_param<W, VE>(weight, c, w);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          const float z = (f[i] - mean[r]) * rstd[r];
+          f[i] = rstd[r] * (fmaf(g[i], w[i], -m0) - z * m1);
+        }
+        ds[c] = X::pack(f);
+      }
+    }
+  }
+  if (partial == nullptr) return;
+  float* p = partial + (int64_t)blockIdx.x * 2 * hidden;
+#pragma unroll
+  for (int q = 0; q < CH; ++q) {
+    const int c = q * NT + tid;
+    if (c >= vecs) continue;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) { p[c * VE + i] = dw[q][i]; p[hidden + c * VE + i] = db[q][i]; }
+  }
+}
+
+constexpr int LN_MAX_PARTS = 592;
+static int64_t ln_parts(int64_t n_rows) { return n_rows < LN_MAX_PARTS ? n_rows : LN_MAX_PARTS; }
+
+// the widest access that rows of `hidden` elements of `size` bytes allow at these addresses; strides in elements (0: one row)
+static int ln_access(int hidden, int size, int wsize, int64_t s0, int64_t s1, const void* a, const void* b, const void* c, const void* w,
+                     const void* bias) {
+  const uintptr_t all = (uintptr_t)((int64_t)hidden * size) | (uintptr_t)(s0 * size) | (uintptr_t)(s1 * size) |
+                        reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c);
+  const uintptr_t par = reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(bias);
+  if ((all & 15) == 0 && (par & 15) == 0) return 16 / size;
+  if (size == 2 && (all & 3) == 0 && (par & (2 * wsize - 1)) == 0) return 2;
+  return 1;
+}
+
 // ---- any hidden size: one block per row, the row re-read from L1 / L2 for each pass ----------------------------
 constexpr int LN_T = 256;
 
@@ -117,16 +374,91 @@ layernorm_dparam_kernel(const float* __restrict__ partial, int n_parts, int hidd
   }
 }
 
-constexpr int LN_MAX_PARTS = 592;
-static int64_t ln_parts(int64_t n_rows) { return n_rows < LN_MAX_PARTS ? n_rows : LN_MAX_PARTS; }
+template <typename T, typename W, int VE>
+static int layernorm_fwd_v(const void* x, int64_t x_stride, const void* weight, const void* bias, float eps, int64_t n_rows,
+                           int hidden, void* out, float* mean, float* rstd, cudaStream_t st) {
+  const int vecs = hidden / VE;
+#define BIBO_LN_FWD(G, CH)                                                                                                       \
+  layernorm_kernel<T, W, VE, G, CH><<<(unsigned)(G > 32 ? n_rows : (n_rows + 7) / 8), G > 32 ? G : 256, 0, st>>>(                \
+      static_cast<const T*>(x), x_stride, static_cast<const W*>(weight), static_cast<const W*>(bias), eps, n_rows, hidden,       \
+      static_cast<T*>(out), mean, rstd)
+  // A warp per row keeps eight loads a lane in flight and needs no barrier; a block per row where the row is longer than
+  // that, or where the rows are too few to fill the machine with warps (8 x 2048 bf16: 2.3 us against 3.3 us).
+  const bool few = n_rows <= 4 * (int64_t)sm_count() && vecs > 64;
+  if (!few && vecs <= 64) BIBO_LN_FWD(32, 2);
+  else if (!few && vecs <= 128) BIBO_LN_FWD(32, 4);
+  else if (!few && vecs <= 256) BIBO_LN_FWD(32, 8);
+  else if (vecs <= 64) BIBO_LN_FWD(32, 2);
+  else if (vecs <= 256) BIBO_LN_FWD(256, 1);
+  else if (vecs <= 512) BIBO_LN_FWD(256, 2);
+  else if (vecs <= 1024) BIBO_LN_FWD(256, 4);
+  else if (vecs <= 2048) BIBO_LN_FWD(256, 8);
+  else if (vecs <= 8192) BIBO_LN_FWD(1024, 8);
+  else
+    layernorm_loop_kernel<T, W><<<(unsigned)n_rows, LN_T, 0, st>>>(
+        static_cast<const T*>(x), x_stride, static_cast<const W*>(weight), static_cast<const W*>(bias), eps, hidden,
+        static_cast<T*>(out), mean, rstd);
+#undef BIBO_LN_FWD
+  BIBO_CHECK_LAUNCH("layernorm_kernel");
+  return BIBO_OK;
+}
 
 template <typename T, typename W>
 static int layernorm_fwd_t(const void* x, int64_t x_stride, const void* weight, const void* bias, float eps, int64_t n_rows,
                            int hidden, void* out, float* mean, float* rstd, cudaStream_t st) {
-  layernorm_loop_kernel<T, W><<<(unsigned)n_rows, LN_T, 0, st>>>(
-      static_cast<const T*>(x), x_stride, static_cast<const W*>(weight), static_cast<const W*>(bias), eps, hidden,
-      static_cast<T*>(out), mean, rstd);
-  BIBO_CHECK_LAUNCH("layernorm_loop_kernel");
+  const int ve = ln_access(hidden, sizeof(T), sizeof(W), n_rows > 1 ? x_stride : 0, 0, x, out, nullptr, weight, bias);
+  if constexpr (sizeof(T) == 2) {
+    if (ve == 8) return layernorm_fwd_v<T, W, 8>(x, x_stride, weight, bias, eps, n_rows, hidden, out, mean, rstd, st);
+    if (ve == 2) return layernorm_fwd_v<T, W, 2>(x, x_stride, weight, bias, eps, n_rows, hidden, out, mean, rstd, st);
+  } else {
+    if (ve == 4) return layernorm_fwd_v<T, W, 4>(x, x_stride, weight, bias, eps, n_rows, hidden, out, mean, rstd, st);
+  }
+  return layernorm_fwd_v<T, W, 1>(x, x_stride, weight, bias, eps, n_rows, hidden, out, mean, rstd, st);
+}
+
+template <typename T, typename W, int VE, int NT, int CH, int R>
+static int layernorm_bwd_v(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
+                           const float* mean, const float* rstd, int64_t n_rows, int hidden, void* dx, float* partial,
+                           int* parts, cudaStream_t st) {
+  auto kern = layernorm_bwd_kernel<T, W, VE, NT, CH, R>;
+  static DeviceOnce once;
+  int per_sm = 1;
+  const int rc = once.get([&](int* v) {
+    BIBO_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(v, kern, NT, 0));
+    return (int)BIBO_OK;
+  }, &per_sm);
+  if (rc) return rc;
+  int64_t grid = (n_rows + R - 1) / R;
+  const int64_t fit = (int64_t)sm_count() * (per_sm > 0 ? per_sm : 1);
+  if (grid > fit) grid = fit;
+  if (grid > LN_MAX_PARTS) grid = LN_MAX_PARTS;
+  kern<<<(unsigned)grid, NT, 0, st>>>(static_cast<const T*>(x), x_stride, static_cast<const T*>(dy), dy_stride,
+                                      static_cast<const W*>(weight), mean, rstd, n_rows, hidden, static_cast<T*>(dx), partial);
+  BIBO_CHECK_LAUNCH("layernorm_bwd_kernel");
+  *parts = (int)grid;
+  return BIBO_OK;
+}
+
+// columns per thread and rows per group: as many loads in flight as the registers hold beside the 2 CH VE column sums
+template <typename T, typename W, int VE>
+static int layernorm_bwd_pick(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
+                              const float* mean, const float* rstd, int64_t n_rows, int hidden, void* dx, float* partial,
+                              int* parts, bool* done, cudaStream_t st) {
+  const int vecs = hidden / VE;
+  *done = true;
+#define BIBO_LN_BWD(NT, CH, R)                                                                                              \
+  return layernorm_bwd_v<T, W, VE, NT, CH, R>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, partial, parts, st)
+  if (vecs <= 64) BIBO_LN_BWD(64, 1, 8);
+  if (vecs <= 128) BIBO_LN_BWD(128, 1, 4);
+  if (vecs <= 256) BIBO_LN_BWD(256, 1, 4);
+  if (vecs <= 512) BIBO_LN_BWD(256, 2, 2);
+  if (vecs <= 1024) BIBO_LN_BWD(512, 2, 2);
+  if (vecs <= 2048) BIBO_LN_BWD(512, 4, 1);
+  if constexpr (VE < 8) {
+    if (vecs <= 4096) BIBO_LN_BWD(512, 8, 1);
+  }
+#undef BIBO_LN_BWD
+  *done = false;
   return BIBO_OK;
 }
 
@@ -134,16 +466,30 @@ template <typename T, typename W>
 static int layernorm_bwd_t(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
                            const float* mean, const float* rstd, int64_t n_rows, int hidden, void* dx, float* partial,
                            void* dweight, void* dbias, cudaStream_t st) {
-  layernorm_bwd_dx_loop_kernel<T, W><<<(unsigned)n_rows, LN_T, 0, st>>>(
-      static_cast<const T*>(x), x_stride, static_cast<const T*>(dy), dy_stride, static_cast<const W*>(weight), mean, rstd,
-      hidden, static_cast<T*>(dx));
-  BIBO_CHECK_LAUNCH("layernorm_bwd_dx_loop_kernel");
-  if (dweight == nullptr && dbias == nullptr) return BIBO_OK;
-  const int64_t parts = ln_parts(n_rows), per = (n_rows + parts - 1) / parts;
-  const int used = (int)((n_rows + per - 1) / per);
-  layernorm_bwd_cols_kernel<T><<<dim3(used, (hidden + LN_T - 1) / LN_T), LN_T, 0, st>>>(
-      static_cast<const T*>(x), x_stride, static_cast<const T*>(dy), dy_stride, mean, rstd, n_rows, hidden, per, partial);
-  BIBO_CHECK_LAUNCH("layernorm_bwd_cols_kernel");
+  const bool params = dweight != nullptr || dbias != nullptr;
+  const int ve = ln_access(hidden, sizeof(T), sizeof(W), n_rows > 1 ? x_stride : 0, n_rows > 1 ? dy_stride : 0, x, dy, dx, weight,
+                           nullptr);
+  int used = 0, rc = BIBO_OK;
+  bool done = false;
+  float* part = params ? partial : nullptr;
+#define BIBO_LN_PICK(VE) layernorm_bwd_pick<T, W, VE>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, part, &used, &done, st)
+  if constexpr (sizeof(T) == 2) rc = ve == 8 ? BIBO_LN_PICK(8) : ve == 2 ? BIBO_LN_PICK(2) : BIBO_LN_PICK(1);
+  else rc = ve == 4 ? BIBO_LN_PICK(4) : BIBO_LN_PICK(1);
+#undef BIBO_LN_PICK
+  if (rc) return rc;
+  if (!done) {                                   // rows too long for the registers of a block
+    layernorm_bwd_dx_loop_kernel<T, W><<<(unsigned)n_rows, LN_T, 0, st>>>(
+        static_cast<const T*>(x), x_stride, static_cast<const T*>(dy), dy_stride, static_cast<const W*>(weight), mean, rstd,
+        hidden, static_cast<T*>(dx));
+    BIBO_CHECK_LAUNCH("layernorm_bwd_dx_loop_kernel");
+    if (!params) return BIBO_OK;
+    const int64_t parts = ln_parts(n_rows), per = (n_rows + parts - 1) / parts;
+    used = (int)((n_rows + per - 1) / per);
+    layernorm_bwd_cols_kernel<T><<<dim3(used, (hidden + LN_T - 1) / LN_T), LN_T, 0, st>>>(
+        static_cast<const T*>(x), x_stride, static_cast<const T*>(dy), dy_stride, mean, rstd, n_rows, hidden, per, partial);
+    BIBO_CHECK_LAUNCH("layernorm_bwd_cols_kernel");
+  }
+  if (!params) return BIBO_OK;
   layernorm_dparam_kernel<W><<<dim3((hidden + 31) / 32, 2), 256, 0, st>>>(partial, used, hidden, static_cast<W*>(dweight),
                                                                         static_cast<W*>(dbias));
   BIBO_CHECK_LAUNCH("layernorm_dparam_kernel");
