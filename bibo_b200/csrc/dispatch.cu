@@ -8,15 +8,12 @@
 //             dw[t,j] = <ys[slot_row[t,j]], dout[t]>, other rows of dys zero
 // A negative index is an empty slot: it has no row, its weight is not read and its dw is 0.  An index >= E is treated
 // the same way and raises the plan's status word.  Sums are fp32 in slot order: results do not depend on timing.
-#include <cooperative_groups.h>
-
 #include "common.cuh"
 
 namespace bibo {
 
-namespace cg = cooperative_groups;
-
-// words of the plan buffer: offsets [E+1], counts [E], status, then (16-byte aligned) slot_row [slots], row_slot [rows]
+// words of the plan buffer: offsets [E+1], counts [E], status, then (16-byte aligned) slot_row [slots], row_slot [rows] and, for
+// more slots than one block sorts, scratch [blocks][E+1]
 __host__ __device__ inline int64_t dp_off_counts(int E) { return E + 1; }
 __host__ __device__ inline int64_t dp_off_status(int E) { return 2 * (int64_t)E + 1; }
 __host__ __device__ inline int64_t dp_off_slot_row(int E) { return (2 * (int64_t)E + 2 + 3) / 4 * 4; }
@@ -25,112 +22,209 @@ inline int64_t dp_rows_cap(int64_t slots, int E, int align) {
   const int64_t groups = slots < E ? slots : E;
   return (slots + groups * (align - 1) + align - 1) / align * align;
 }
+constexpr int DP_ONE_BLOCK = 8192, DP_MAX_BLOCKS = 256;     // slots that one block sorts; blocks for more
+inline int64_t dp_blocks(int64_t slots) {
+  if (slots <= DP_ONE_BLOCK) return 0;
+  const int64_t b = (slots + 1023) / 1024;
+  return b < DP_MAX_BLOCKS ? b : DP_MAX_BLOCKS;
+}
+inline int64_t dp_off_scratch(int64_t slots, int E, int64_t rows_cap) { return dp_off_row_slot(E, slots) + (rows_cap + 3) / 4 * 4; }
 constexpr int DP_MAX_EXPERTS = 1024, DP_MAX_TOP_K = 32, DP_STATUS_INDEX = 2;
 
-// ---- plan: a stable counting sort in one launch ------------------------------------------------------------------
-// One cluster.  Each warp owns a contiguous range of slots and a histogram row in shared memory; the warp totals are
-// scanned per expert inside the block, the block totals across the cluster through distributed shared memory, and a
-// second pass over the (L2-resident) indices hands out the rows in slot order.
+// ---- plan: a stable counting sort -------------------------------------------------------------------------------
+// Each warp owns a contiguous range of slots and a histogram in shared memory.  A slot's rank among the warp's slots of its
+// expert comes from one ballot per index bit; a scan over the block's warps makes it the rank in the block, which waits in
+// slot_row.  Up to DP_ONE_BLOCK slots one block does everything.  Above that a first launch ranks inside blocks of >= 1024 slots and
+// leaves their counts, and in a second one every block adds up the counts of the blocks below it (L2-resident), the
+// offsets, and its ranks.  (One cluster of 16 blocks with the counts exchanged through distributed shared memory took 30 us for
+// 196608 slots: the scattered stores of row_slot want more than 16 SMs.)
+constexpr int DP_BATCH = 8;        // index loads in flight per lane
+
+struct DpBlock {                   // shared memory of a block
+  int32_t *offset, *count, *lower, *hists;      // [E+1], [E], [E], [warps][pitch]
+  int pitch;
+  __device__ DpBlock(int32_t* sm, int E) : offset(sm), count(sm + E + 1), lower(sm + 2 * E + 1), hists(sm + 3 * E + 1), pitch(E | 1) {}
+};
+static size_t dp_smem(int E, int threads) { return sizeof(int32_t) * (3 * (size_t)E + 1 + (size_t)(threads / 32) * (E | 1)); }
+
+template <typename I> __device__ __forceinline__ int dp_expert(const I* idx, int64_t s, int64_t end, int E, int* bad) {
+  if (s >= end) return -1;
+  const int64_t v = (int64_t)idx[s];
+  if (v >= E) *bad = 1;
+  return v >= 0 && v < E ? (int)v : -1;
+}
+// ranks of the slots [s0, s1) of this warp inside the warp into slot_row (-1: no slot), and its histogram
 template <typename I>
-__global__ void __launch_bounds__(1024, 1)
-dispatch_plan_kernel(const I* __restrict__ idx, int64_t slots, int E, int align, int64_t rows_cap, int32_t* __restrict__ plan) {
-  extern __shared__ int32_t sm[];
-  const int warps = blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  cg::cluster_group cl = cg::this_cluster();
-  const int cta = (int)cl.block_rank(), n_cta = (int)cl.num_blocks();
-  int32_t* total = sm;                       // [E]   this block's slots per expert (read by the other blocks)
-  int32_t* base = sm + E;                    // [E+1] first row of this block's slots of an expert; before that the offsets
-  int32_t* hist = sm + 2 * E + 1 + (size_t)warp * E;
-  int32_t* slot_row = plan + dp_off_slot_row(E);
-  int32_t* row_slot = plan + dp_off_row_slot(E, slots);
+__device__ __forceinline__ void dp_rank(const I* __restrict__ idx, int64_t s0, int64_t s1, int E, int bits, int32_t* hist,
+                                        int32_t* __restrict__ slot_row, int* bad) {
+  const int lane = threadIdx.x & 31;
   for (int e = lane; e < E; e += 32) hist[e] = 0;
   __syncwarp();
-  const int64_t n_warps = (int64_t)n_cta * warps, per = ((slots + n_warps - 1) / n_warps + 31) / 32 * 32;
-  const int64_t s0 = ((int64_t)cta * warps + warp) * per, s1 = s0 + per < slots ? s0 + per : slots;
-  bool bad = false;
-  for (int64_t s = s0; s < s1; s += 32) {
-    const int64_t v = s + lane < s1 ? (int64_t)idx[s + lane] : -1;
-    const int e = v >= 0 && v < E ? (int)v : -1;
-    bad |= v >= E;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    if (e >= 0 && lane == __ffs(same) - 1) hist[e] += __popc(same);
-    __syncwarp();
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < E; e += blockDim.x) {     // exclusive scan over the warps of this block
-    int run = 0;
-    for (int w = 0; w < warps; ++w) {
-      int32_t* h = sm + 2 * E + 1 + (size_t)w * E + e;
-      const int c = *h;
-      *h = run;
-      run += c;
-    }
-    total[e] = run;
-  }
-  cl.sync();
-  // every block: counts over the cluster and the slots of lower blocks
-  for (int e = threadIdx.x; e < E; e += blockDim.x) {
-    int all = 0, lower = 0;
-    for (int b = 0; b < n_cta; ++b) {
-      const int c = cl.map_shared_rank(total, b)[e];
-      all += c;
-      if (b < cta) lower += c;
-    }
-    base[e] = all;
-    if (cta == 0) plan[dp_off_counts(E) + e] = all;
-    for (int w = 0; w < warps; ++w) sm[2 * E + 1 + (size_t)w * E + e] += lower;
-  }
-  __syncthreads();
-  if (warp == 0) {                                          // offsets: exclusive scan of the padded counts
-    int carry = 0;
-    for (int e0 = 0; e0 < E; e0 += 32) {
-      const int e = e0 + lane;
-      const int c = e < E ? (base[e] + align - 1) / align * align : 0;
-      int inc = c;
+  for (int64_t b0 = s0; b0 < s1; b0 += 32 * DP_BATCH) {
+    int ex[DP_BATCH];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
-      if (e < E) base[e] = carry + inc - c;
-      carry += __shfl_sync(0xffffffffu, inc, 31);
+    for (int i = 0; i < DP_BATCH; ++i) ex[i] = dp_expert(idx, b0 + i * 32 + lane, s1, E, bad);
+#pragma unroll
+    for (int i = 0; i < DP_BATCH; ++i) {
+      if (b0 + i * 32 >= s1) break;          // the whole warp
+      const int e = ex[i];
+      unsigned same = __ballot_sync(0xffffffffu, e >= 0);
+      for (int bit = 0; bit < bits; ++bit) {
+        const unsigned one = __ballot_sync(0xffffffffu, (e >> bit) & 1);
+        same &= (e >> bit) & 1 ? one : ~one;
+      }
+      int rank = -1;
+      if (e >= 0) rank = hist[e] + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (e >= 0 && (same >> lane) == 1u) hist[e] = rank + 1;       // the last lane of the expert
+      __syncwarp();
+      if (b0 + i * 32 + lane < s1) slot_row[b0 + i * 32 + lane] = rank;
     }
-    if (lane == 0) base[E] = carry;
+  }
+}
+// hists: exclusive scan over the warps of the block; count: the block's slots of each expert
+__device__ __forceinline__ void dp_scan_warps(const DpBlock& d, int E) {
+  const int warps = blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = warp; e < E; e += warps) {
+    const int c = lane < warps ? d.hists[(size_t)lane * d.pitch + e] : 0;
+    int inc = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
+    if (lane < warps) d.hists[(size_t)lane * d.pitch + e] = inc - c;
+    if (lane == 31) d.count[e] = inc;
+  }
+}
+// offsets from the counts: exclusive scan of the counts rounded up to `align`; one warp
+__device__ __forceinline__ void dp_offsets(const DpBlock& d, int E, int align) {
+  const int lane = threadIdx.x & 31;
+  int carry = 0;
+  for (int e0 = 0; e0 < E; e0 += 32) {
+    const int e = e0 + lane;
+    const int c = e < E ? (d.count[e] + align - 1) / align * align : 0;
+    int inc = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += t; }
+    if (e < E) d.offset[e] = carry + inc - c;
+    carry += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (lane == 0) d.offset[E] = carry;
+}
+// rows without a slot: the padding behind each group and everything behind the last group; block `b` of `n`
+__device__ __forceinline__ void dp_free_rows(const DpBlock& d, int E, int align, int64_t rows_cap, int b, int n, int32_t* row_slot) {
+  const int warps = blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (align > 1)
+    for (int e = b * warps + warp; e < E; e += n * warps)
+      for (int r = d.offset[e] + d.count[e] + lane; r < d.offset[e + 1]; r += 32) row_slot[r] = -1;
+  for (int64_t r = d.offset[E] + (int64_t)b * blockDim.x + threadIdx.x; r < rows_cap; r += (int64_t)n * blockDim.x) row_slot[r] = -1;
+}
+__device__ __forceinline__ void dp_write_head(const DpBlock& d, int E, int bad, int32_t* plan) {
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) {
+    plan[e] = d.offset[e];
+    if (e < E) plan[dp_off_counts(E) + e] = d.count[e];
+  }
+  if (threadIdx.x == 0) plan[dp_off_status(E)] = bad ? DP_STATUS_INDEX : 0;
+}
+
+template <typename I>
+__global__ void __launch_bounds__(1024)
+dispatch_plan_kernel(const I* __restrict__ idx, int64_t slots, int E, int bits, int align, int64_t rows_cap, int32_t* __restrict__ plan) {
+  extern __shared__ int32_t sm[];
+  __shared__ int bad_s;
+  const DpBlock d(sm, E);
+  const int warps = blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int32_t* hist = d.hists + (size_t)warp * d.pitch;
+  int32_t* slot_row = plan + dp_off_slot_row(E);
+  int32_t* row_slot = plan + dp_off_row_slot(E, slots);
+  if (threadIdx.x == 0) bad_s = 0;
+  __syncthreads();
+  const int64_t per = ((slots + warps - 1) / warps + 31) / 32 * 32, s0 = min(slots, warp * per), s1 = min(slots, s0 + per);
+  dp_rank(idx, s0, s1, E, bits, hist, slot_row, &bad_s);
+  __syncthreads();
+  dp_scan_warps(d, E);
+  __syncthreads();
+  if (warp == 0) dp_offsets(d, E, align);
+  __syncthreads();
+  dp_write_head(d, E, bad_s, plan);
+  dp_free_rows(d, E, align, rows_cap, 0, 1, row_slot);
+  for (int64_t s = s0 + lane; s < s1; s += 32) {
+    const int rank = slot_row[s];                              // written by this lane
+    if (rank < 0) continue;
+    const int e = (int)idx[s], row = d.offset[e] + hist[e] + rank;
+    slot_row[s] = row;
+    row_slot[row] = (int32_t)s;
+  }
+}
+
+// more slots: ranks inside a block's slots, and its counts in scratch [blocks][E] (flags behind them)
+template <typename I>
+__global__ void __launch_bounds__(1024)
+dispatch_count_kernel(const I* __restrict__ idx, int64_t slots, int64_t per_block, int E, int bits, int32_t* __restrict__ slot_row,
+                      int32_t* __restrict__ scratch) {
+  extern __shared__ int32_t sm[];
+  __shared__ int bad_s;
+  const DpBlock d(sm, E);
+  const int warps = blockDim.x / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int32_t* hist = d.hists + (size_t)warp * d.pitch;
+  if (threadIdx.x == 0) bad_s = 0;
+  __syncthreads();
+  const int64_t b0 = min(slots, blockIdx.x * per_block), b1 = min(slots, b0 + per_block);
+  const int64_t per = ((b1 - b0 + warps - 1) / warps + 31) / 32 * 32, s0 = min(b1, b0 + warp * per), s1 = min(b1, s0 + per);
+  dp_rank(idx, s0, s1, E, bits, hist, slot_row, &bad_s);
+  __syncthreads();
+  dp_scan_warps(d, E);
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += blockDim.x) scratch[(int64_t)blockIdx.x * E + e] = d.count[e];
+  if (threadIdx.x == 0) scratch[(int64_t)gridDim.x * E + blockIdx.x] = bad_s;
+  for (int64_t s = s0 + lane; s < s1; s += 32) {
+    const int rank = slot_row[s];
+    if (rank >= 0) slot_row[s] = rank + hist[(int)idx[s]];
+  }
+}
+// ... and the rows: every block adds up the counts of the blocks below its own
+template <typename I>
+__global__ void __launch_bounds__(1024)
+dispatch_rows_kernel(const I* __restrict__ idx, int64_t slots, int64_t per_block, int E, int align, int64_t rows_cap,
+                     const int32_t* __restrict__ scratch, int32_t* __restrict__ plan) {
+  extern __shared__ int32_t sm[];
+  const DpBlock d(sm, E);
+  const int n = gridDim.x, b = blockIdx.x;
+  for (int e = threadIdx.x; e < E; e += blockDim.x) d.count[e] = d.lower[e] = 0;
+  __syncthreads();
+  // a thread adds up one expert over every `groups`-th block, then once into shared memory (whole numbers: any order)
+  int ep = 32;
+  while (ep < E) ep *= 2;
+  const int groups = blockDim.x / ep, e = threadIdx.x % ep;
+  if (e < E) {
+    int all = 0, low = 0;
+#pragma unroll 8
+    for (int at = threadIdx.x / ep; at < n; at += groups) {
+      const int c = scratch[(int64_t)at * E + e];
+      all += c;
+      low += at < b ? c : 0;
+    }
+    atomicAdd(&d.count[e], all);
+    atomicAdd(&d.lower[e], low);
   }
   __syncthreads();
-  if (cta == 0) {
-    for (int e = threadIdx.x; e <= E; e += blockDim.x) plan[e] = base[e];
-  }
-  // rows without a slot: the padding behind each group and everything behind the last group
-  for (int e = cta * warps + warp; e < E; e += n_cta * warps) {
-    int all = 0;
-    for (int b = 0; b < n_cta; ++b) all += cl.map_shared_rank(total, b)[e];
-    for (int r = base[e] + all + lane; r < base[e + 1]; r += 32) row_slot[r] = -1;
-  }
-  for (int64_t r = base[E] + (int64_t)cta * blockDim.x + threadIdx.x; r < rows_cap; r += (int64_t)n_cta * blockDim.x)
-    row_slot[r] = -1;
-  for (int64_t s = s0; s < s1; s += 32) {
-    const bool in = s + lane < s1;
-    const int64_t v = in ? (int64_t)idx[s + lane] : -1;
-    const int e = v >= 0 && v < E ? (int)v : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    int row = -1;
-    if (e >= 0) row = base[e] + hist[e] + __popc(same & ((1u << lane) - 1));
-    __syncwarp();
-    if (e >= 0 && lane == __ffs(same) - 1) hist[e] += __popc(same);
-    __syncwarp();
-    if (in) slot_row[s + lane] = row;
-    if (row >= 0) row_slot[row] = (int32_t)(s + lane);
-  }
-  // the status word: raised by any block, written once by block 0 after every block has looked at its slots
-  __shared__ int bad_here;
-  if (threadIdx.x == 0) bad_here = 0;
+  if (threadIdx.x < 32) dp_offsets(d, E, align);
   __syncthreads();
-  if (bad) bad_here = 1;
-  cl.sync();
-  if (cta == 0 && threadIdx.x == 0) {
-    int any = 0;
-    for (int b = 0; b < n_cta; ++b) any |= *cl.map_shared_rank(&bad_here, b);
-    plan[dp_off_status(E)] = any ? DP_STATUS_INDEX : 0;
+  int32_t* slot_row = plan + dp_off_slot_row(E);
+  int32_t* row_slot = plan + dp_off_row_slot(E, slots);
+  if (b == 0) {
+    int bad = 0;
+    if (threadIdx.x == 0)
+      for (int i = 0; i < n; ++i) bad |= scratch[(int64_t)n * E + i];
+    dp_write_head(d, E, bad, plan);
   }
-  cl.sync();                                                // no block leaves while its shared memory is read
+  dp_free_rows(d, E, align, rows_cap, b, n, row_slot);
+  const int64_t s0 = min(slots, b * per_block), s1 = min(slots, s0 + per_block);
+  for (int64_t s = s0 + threadIdx.x; s < s1; s += blockDim.x) {
+    const int rank = slot_row[s];
+    if (rank < 0) continue;
+    const int ex = (int)idx[s], row = d.offset[ex] + d.lower[ex] + rank;
+    slot_row[s] = row;
+    row_slot[row] = (int32_t)s;
+  }
 }
 
 // ---- row copies and sums, by the widest access that the rows' alignment allows ------------------------------------
@@ -397,30 +491,31 @@ static int row_parts(int64_t n_tokens, int chunks, int* part) {
 }
 
 template <typename I>
-static int plan_launch(const void* idx, int64_t slots, int E, int align, int32_t* plan, cudaStream_t st) {
-  auto kern = dispatch_plan_kernel<I>;
+static int plan_launch(const void* idx_, int64_t slots, int E, int align, int32_t* plan, cudaStream_t st) {
   static DeviceOnce once;
   const int rc = once.get([&](int*) {
-    BIBO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(int32_t) * (34 * DP_MAX_EXPERTS + 1)));
+    BIBO_CUDA(cudaFuncSetAttribute(dispatch_plan_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dp_smem(DP_MAX_EXPERTS, 1024)));
+    BIBO_CUDA(cudaFuncSetAttribute(dispatch_count_kernel<I>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dp_smem(DP_MAX_EXPERTS, 1024)));
     return (int)BIBO_OK;
   });
   if (rc) return rc;
-  // one block up to 8192 slots (a cluster barrier costs more than the eighth of the work that it saves), eight above
-  const int blocks = slots <= 8192 ? 1 : 8;
-  const int threads = slots <= 1024 ? 256 : 1024;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = sizeof(int32_t) * (2 * (size_t)E + 1 + (size_t)(threads / 32) * E);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = blocks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  BIBO_CUDA(cudaLaunchKernelEx(&cfg, kern, static_cast<const I*>(idx), slots, E, align, dp_rows_cap(slots, E, align), plan));
-  BIBO_CHECK_LAUNCH("dispatch_plan_kernel");
+  const I* idx = static_cast<const I*>(idx_);
+  int bits = 0;
+  while ((1 << bits) < E) ++bits;
+  const int64_t cap = dp_rows_cap(slots, E, align);
+  const int blocks = (int)dp_blocks(slots);
+  if (blocks == 0) {
+    const int threads = slots <= 1024 ? 256 : 1024;
+    dispatch_plan_kernel<I><<<1, threads, dp_smem(E, threads), st>>>(idx, slots, E, bits, align, cap, plan);
+    BIBO_CHECK_LAUNCH("dispatch_plan_kernel");
+    return BIBO_OK;
+  }
+  const int64_t per = (slots + blocks - 1) / blocks;
+  int32_t* scratch = plan + dp_off_scratch(slots, E, cap);
+  dispatch_count_kernel<I><<<blocks, 1024, dp_smem(E, 1024), st>>>(idx, slots, per, E, bits, plan + dp_off_slot_row(E), scratch);
+  BIBO_CHECK_LAUNCH("dispatch_count_kernel");
+  dispatch_rows_kernel<I><<<blocks, 1024, dp_smem(E, 0), st>>>(idx, slots, per, E, align, cap, scratch, plan);
+  BIBO_CHECK_LAUNCH("dispatch_rows_kernel");
   return BIBO_OK;
 }
 
@@ -434,7 +529,8 @@ extern "C" int64_t bibo_moe_dispatch_rows_cap(int64_t n_tokens, int top_k, int n
 }
 extern "C" int64_t bibo_moe_dispatch_plan_words(int64_t n_tokens, int top_k, int n_experts, int align) {
   if (dispatch_check("dispatch_plan_words", n_tokens, 1, n_experts, top_k, align, BIBO_F32)) return -1;
-  return dp_off_row_slot(n_experts, n_tokens * top_k) + dp_rows_cap(n_tokens * top_k, n_experts, align);
+  const int64_t slots = n_tokens * top_k;
+  return dp_off_scratch(slots, n_experts, dp_rows_cap(slots, n_experts, align)) + dp_blocks(slots) * (n_experts + 1);
 }
 extern "C" int64_t bibo_moe_dispatch_off_slot_row(int n_experts) { return dp_off_slot_row(n_experts); }
 extern "C" int64_t bibo_moe_dispatch_off_row_slot(int64_t n_tokens, int top_k, int n_experts) {

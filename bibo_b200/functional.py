@@ -6,6 +6,7 @@ one workspace per shape) and passes their raw pointers through ctypes.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 from typing import Dict, Optional, Tuple
 
@@ -419,6 +420,18 @@ def experts_forward(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tenso
     return out, ws
 
 
+@functools.lru_cache(maxsize=1024)
+def _plan_layout(n_tokens: int, top_k: int, n_experts: int, align: int) -> Tuple[int, int, int, int]:
+    """(rows, words, word of slot_row, word of row_slot) of a plan of these sizes."""
+    lib = _lib.load()
+    rows = int(lib.bibo_moe_dispatch_rows_cap(n_tokens, top_k, n_experts, align))
+    if rows < 0:
+        raise RuntimeError("dispatch plan: " + lib.bibo_moe_last_error_string().decode(errors="replace"))
+    return (rows, int(lib.bibo_moe_dispatch_plan_words(n_tokens, top_k, n_experts, align)),
+            int(lib.bibo_moe_dispatch_off_slot_row(n_experts)),
+            int(lib.bibo_moe_dispatch_off_row_slot(n_tokens, top_k, n_experts)))
+
+
 class DispatchPlan:
     """Row order of one routing (bibo_moe_dispatch_plan): the slots of ``topk_idx`` sorted by expert, in slot order within
     an expert.  ``rows`` is the number of rows of an expert-ordered buffer (a bound that the host knows); the device knows
@@ -431,13 +444,9 @@ class DispatchPlan:
     """
 
     def __init__(self, n_tokens: int, top_k: int, n_experts: int, align: int, device):
-        lib = _lib.load()
         self.n_tokens, self.top_k, self.n_experts, self.align = n_tokens, top_k, n_experts, align
-        self.rows = int(lib.bibo_moe_dispatch_rows_cap(n_tokens, top_k, n_experts, align))
-        if self.rows < 0:
-            raise RuntimeError("dispatch plan: " + lib.bibo_moe_last_error_string().decode(errors="replace"))
-        self.buf = torch.empty(int(lib.bibo_moe_dispatch_plan_words(n_tokens, top_k, n_experts, align)), dtype=torch.int32,
-                               device=device)
+        self.rows, words, self._slot_row, self._row_slot = _plan_layout(n_tokens, top_k, n_experts, align)
+        self.buf = torch.empty(words, dtype=torch.int32, device=device)
 
     @property
     def offsets(self) -> torch.Tensor:
@@ -449,13 +458,11 @@ class DispatchPlan:
 
     @property
     def slot_row(self) -> torch.Tensor:
-        o = int(_lib.load().bibo_moe_dispatch_off_slot_row(self.n_experts))
-        return self.buf[o:o + self.n_tokens * self.top_k].view(self.n_tokens, self.top_k)
+        return self.buf.as_strided((self.n_tokens, self.top_k), (self.top_k, 1), self._slot_row)
 
     @property
     def row_slot(self) -> torch.Tensor:
-        o = int(_lib.load().bibo_moe_dispatch_off_row_slot(self.n_tokens, self.top_k, self.n_experts))
-        return self.buf[o:o + self.rows]
+        return self.buf[self._row_slot:self._row_slot + self.rows]
 
     def raise_if_failed(self) -> None:
         """Waits for the plan and raises RuntimeError if an expert index was out of range (such slots count as empty)."""
@@ -472,21 +479,24 @@ def dispatch_plan(topk_idx: torch.Tensor, n_experts: int, align: int = 1) -> Dis
     if topk_idx.dim() != 2 or topk_idx.dtype not in (torch.int32, torch.int64):
         raise RuntimeError(f"topk_idx must be int32 or int64 [N, k], got {topk_idx.dtype} {tuple(topk_idx.shape)}")
     n, k = topk_idx.shape
-    plan = DispatchPlan(n, k, int(n_experts), int(align), topk_idx.device)
-    _launch("bibo_moe_dispatch_plan", topk_idx.device, _lib.ptr(topk_idx), topk_idx.element_size(), n, k, plan.n_experts,
-            plan.align, _lib.ptr(plan.buf))
+    dev = topk_idx.device
+    plan = DispatchPlan(n, k, int(n_experts), int(align), dev)
+    _launch("bibo_moe_dispatch_plan", dev, topk_idx.data_ptr(), topk_idx.element_size(), n, k, plan.n_experts, plan.align,
+            plan.buf.data_ptr())
     return plan
 
 
-def _need_plan_rows(t: torch.Tensor, name: str, plan: DispatchPlan, rows: int) -> None:
-    _need_rows(t, name)
-    if t.shape[0] != rows:
-        raise RuntimeError(f"{name} has {t.shape[0]} rows, the plan needs {rows}")
+def _plan_rows(t: torch.Tensor, name: str, plan: DispatchPlan, rows: int) -> Tuple[int, int]:
+    """(H, row stride) of a tensor with the rows and the device that the plan needs."""
+    n, hidden, stride = _rows(t, name)
+    if n != rows:
+        raise RuntimeError(f"{name} has {n} rows, the plan needs {rows}")
     if t.device != plan.buf.device:
         raise RuntimeError(f"{name} is on {t.device}, the plan on {plan.buf.device}")
+    return hidden, stride
 
 
-def _need_weights(topk_w: Optional[torch.Tensor], plan: DispatchPlan) -> int:
+def _plan_weights(topk_w: Optional[torch.Tensor], plan: DispatchPlan) -> int:
     if topk_w is None:
         return _lib.F32
     _need_cuda(topk_w, "topk_w")
@@ -498,23 +508,23 @@ def _need_weights(topk_w: Optional[torch.Tensor], plan: DispatchPlan) -> int:
 
 def dispatch_forward(x: torch.Tensor, plan: DispatchPlan) -> torch.Tensor:
     """Token rows x [N,H] in expert order (bibo_moe_dispatch_fwd): xs [plan.rows, H]; rows without a slot are zero."""
-    _need_plan_rows(x, "x", plan, plan.n_tokens)
+    hidden, stride = _plan_rows(x, "x", plan, plan.n_tokens)
     dt = dtype_code(x.dtype)
-    xs = torch.empty((plan.rows, x.shape[1]), dtype=x.dtype, device=x.device)
-    _launch("bibo_moe_dispatch_fwd", x.device, _lib.ptr(x), x.stride(0), _lib.ptr(plan.buf), plan.n_tokens, x.shape[1],
-            plan.top_k, plan.n_experts, plan.align, dt, _lib.ptr(xs))
+    xs = x.new_empty((plan.rows, hidden))
+    _launch("bibo_moe_dispatch_fwd", x.device, x.data_ptr(), stride, plan.buf.data_ptr(), plan.n_tokens, hidden, plan.top_k,
+            plan.n_experts, plan.align, dt, xs.data_ptr())
     return xs
 
 
 def combine_forward(ys: torch.Tensor, topk_w: Optional[torch.Tensor], plan: DispatchPlan) -> torch.Tensor:
     """out[t] = sum over the slots of t of topk_w[t,j] * ys[row of the slot] (bibo_moe_dispatch_combine_fwd), summed in fp32
     in slot order.  ``topk_w`` [N,k] is fp32 or bf16, None for a plain sum; an empty slot's weight is not read."""
-    _need_plan_rows(ys, "ys", plan, plan.rows)
+    hidden, _ = _plan_rows(ys, "ys", plan, plan.rows)
     _need_cuda(ys, "ys")
-    dt, wt = dtype_code(ys.dtype), _need_weights(topk_w, plan)
-    out = torch.empty((plan.n_tokens, ys.shape[1]), dtype=ys.dtype, device=ys.device)
-    _launch("bibo_moe_dispatch_combine_fwd", ys.device, _lib.ptr(ys), _lib.ptr(topk_w), wt, _lib.ptr(plan.buf), plan.n_tokens,
-            ys.shape[1], plan.top_k, plan.n_experts, plan.align, dt, _lib.ptr(out))
+    dt, wt = dtype_code(ys.dtype), _plan_weights(topk_w, plan)
+    out = ys.new_empty((plan.n_tokens, hidden))
+    _launch("bibo_moe_dispatch_combine_fwd", ys.device, ys.data_ptr(), None if topk_w is None else topk_w.data_ptr(), wt,
+            plan.buf.data_ptr(), plan.n_tokens, hidden, plan.top_k, plan.n_experts, plan.align, dt, out.data_ptr())
     return out
 
 
@@ -522,16 +532,15 @@ def combine_backward(dout: torch.Tensor, ys: torch.Tensor, topk_w: Optional[torc
                      need_dw: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Gradients of ``combine_forward`` (bibo_moe_dispatch_combine_bwd): (dys [plan.rows, H] with zeros in the rows without a
     slot, d_topk_w [N,k] in topk_w's dtype or None)."""
-    _need_plan_rows(dout, "dout", plan, plan.n_tokens)
-    _need_plan_rows(ys, "ys", plan, plan.rows)
+    hidden, _ = _plan_rows(ys, "ys", plan, plan.rows)
     _need_cuda(ys, "ys")
-    _need_rows(dout, "dout", ys.shape[1], ys)
-    dt, wt = dtype_code(ys.dtype), _need_weights(topk_w, plan)
+    stride = _rows_like(dout, "dout", plan.n_tokens, hidden, ys)
+    dt, wt = dtype_code(ys.dtype), _plan_weights(topk_w, plan)
     dys = torch.empty_like(ys)
     dw = torch.empty_like(topk_w) if need_dw and topk_w is not None else None
     p = _lib.ptr
-    _launch("bibo_moe_dispatch_combine_bwd", ys.device, p(dout), dout.stride(0), p(ys), p(topk_w), wt, p(plan.buf),
-            plan.n_tokens, ys.shape[1], plan.top_k, plan.n_experts, plan.align, dt, p(dys), p(dw))
+    _launch("bibo_moe_dispatch_combine_bwd", ys.device, p(dout), stride, p(ys), p(topk_w), wt, p(plan.buf), plan.n_tokens, hidden,
+            plan.top_k, plan.n_experts, plan.align, dt, p(dys), p(dw))
     return dys, dw
 
 
@@ -571,37 +580,49 @@ def rmsnorm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, ep
     return dh, dweight
 
 
-def _need_rows(t: torch.Tensor, name: str, hidden: Optional[int] = None, like: Optional[torch.Tensor] = None) -> None:
-    """Rows [N,H] on a CUDA device whose elements are next to each other; the rows themselves may be further apart."""
+def _rows(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
+    """(N, H, row stride) of rows [N,H] on a CUDA device whose elements are next to each other; the rows themselves may be
+    further apart.  Raises otherwise."""
     if not t.is_cuda:
         raise RuntimeError(f"{name} is on {t.device}: the bibo_b200 kernels run only on CUDA devices "
                            "(there is no CPU implementation)")
     if t.dim() != 2 or t.shape[1] < 1:
         raise RuntimeError(f"{name} must be rows [N, H] with H >= 1, got shape {tuple(t.shape)}")
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    n, h = t.shape
+    s0, s1 = t.stride()
+    if (s1 != 1 and h > 1) or (s0 < h and n > 1):
         raise RuntimeError(f"{name} must be contiguous within its rows, which may not overlap (strides {t.stride()})")
-    if hidden is not None and t.shape[1] != hidden:
-        raise RuntimeError(f"{name} has rows of {t.shape[1]} elements, expected {hidden}")
-    if like is not None:
-        _need_like(t, name, like)
+    return n, h, s0
 
 
-def _need_like(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+def _rows_like(t: torch.Tensor, name: str, n: int, h: int, like: torch.Tensor) -> int:
+    """Row stride of a second tensor of rows, of the same shape, type and device as the activations."""
+    rows, hidden, stride = _rows(t, name)
+    if hidden != h:
+        raise RuntimeError(f"{name} has rows of {hidden} elements, expected {h}")
+    if rows != n:
+        raise RuntimeError(f"{name} has {rows} rows, expected {n}")
     if t.dtype != like.dtype:
         raise RuntimeError(f"{name} dtype {t.dtype} != activation dtype {like.dtype}")
     if t.device != like.device:
         raise RuntimeError(f"{name} is on {t.device}, the activations on {like.device}")
+    return stride
 
 
 def _launch(name: str, dev: torch.device, *args) -> None:
     """One C-ABI call on ``dev``'s current stream, with ``dev`` made current for it where another device is."""
     fn = getattr(_lib.load(), name)
     if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, _stream(dev))
+        rc = fn(*args, _raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _stream(dev))
-    _lib.check(rc, name)
+            rc = fn(*args, _raw_stream(dev.index))
+    if rc != 0:
+        _lib.check(rc, name)
+
+
+# the current stream as an address: a tenth of the time of building a Stream object for it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def layernorm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -609,24 +630,23 @@ def layernorm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bi
     """Layer norm of flat rows x [N,H] over H (bibo_moe_layernorm_fwd): ``(x - mean) * rstd * weight + bias``, computed in
     fp32 and rounded once.  The rows may be a slice of a wider tensor.  ``weight`` and ``bias`` [H] are each optional and
     share one dtype, fp32 or that of x.  ``keep=True`` returns ``(out, saved)`` with what ``layernorm_backward`` needs."""
-    _need_rows(x, "x")
-    n, hidden = x.shape
-    wtype = x.dtype
+    n, hidden, stride = _rows(x, "x")
+    wtype = dtype = x.dtype
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
         _need_cuda(t, name)
         if t.shape != (hidden,) or t.device != x.device:
             raise RuntimeError(f"{name} must be [{hidden}] on {x.device}, got {tuple(t.shape)} on {t.device}")
-        if t.dtype not in (x.dtype, torch.float32) or (t is bias and weight is not None and bias.dtype != weight.dtype):
-            raise RuntimeError(f"{name} dtype {t.dtype}: weight and bias are both float32 or both {x.dtype}")
+        if t.dtype not in (dtype, torch.float32) or (t is bias and weight is not None and bias.dtype != weight.dtype):
+            raise RuntimeError(f"{name} dtype {t.dtype}: weight and bias are both float32 or both {dtype}")
         wtype = t.dtype
-    out = torch.empty((n, hidden), dtype=x.dtype, device=x.device)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = torch.empty((2, n), dtype=torch.float32, device=x.device) if keep else None
-    p = _lib.ptr
-    mean = p(stats)
-    _launch("bibo_moe_layernorm_fwd", x.device, p(x), x.stride(0), p(weight), p(bias), float(eps), n, hidden,
-            dtype_code(x.dtype), dtype_code(wtype), p(out), mean, None if stats is None else mean + 4 * n)
+    mean = None if stats is None else stats.data_ptr()
+    _launch("bibo_moe_layernorm_fwd", x.device, x.data_ptr(), stride, None if weight is None else weight.data_ptr(),
+            None if bias is None else bias.data_ptr(), eps, n, hidden, dtype_code(dtype), dtype_code(wtype), out.data_ptr(), mean,
+            None if stats is None else mean + 4 * n)
     return (out, (stats, wtype)) if keep else out
 
 
@@ -635,13 +655,12 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch
     """Gradients of ``layernorm_forward(..., keep=True)`` (bibo_moe_layernorm_bwd): (dx [N,H], dweight [H] or None without
     a weight, dbias [H] or None without a bias).  The sums over the rows are taken in a fixed order."""
     stats, wtype = saved
-    _need_rows(x, "x")
-    n, hidden = x.shape
-    _need_rows(dy, "dy", hidden, x)
-    if dy.shape[0] != n or stats.shape != (2, n):
-        raise RuntimeError(f"dy has {dy.shape[0]} rows and the forward kept {stats.shape[1]}, x has {n}")
+    n, hidden, stride = _rows(x, "x")
+    dy_stride = _rows_like(dy, "dy", n, hidden, x)
+    if stats.shape != (2, n):
+        raise RuntimeError(f"the forward kept {stats.shape[1]} rows, x has {n}")
     dev = x.device
-    dx = torch.empty((n, hidden), dtype=x.dtype, device=dev)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     make = torch.empty if n else torch.zeros                   # sums over no rows
     dweight = make(hidden, dtype=wtype, device=dev) if weight is not None and need_dweight else None
     dbias = make(hidden, dtype=wtype, device=dev) if has_bias else None
@@ -650,7 +669,7 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch
         parts = int(_lib.load().bibo_moe_layernorm_bwd_parts(n))
         partial = torch.empty((parts, 2, hidden), dtype=torch.float32, device=dev)
     p = _lib.ptr
-    _launch("bibo_moe_layernorm_bwd", dev, p(x), x.stride(0), p(dy), dy.stride(0), p(weight), p(stats), p(stats) + 4 * n, n,
+    _launch("bibo_moe_layernorm_bwd", dev, p(x), stride, p(dy), dy_stride, p(weight), p(stats), p(stats) + 4 * n, n,
             hidden, dtype_code(x.dtype), dtype_code(wtype), p(dx), p(partial), p(dweight), p(dbias))
     return dx, dweight, dbias
 
