@@ -330,9 +330,23 @@ __device__ __forceinline__ float load_weight(const void* w, int is_bf16, int64_t
   return is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]) : static_cast<const float*>(w)[i];
 }
 
-// out[t] = sum_j w[t,j] * ys[slot_row[t,j]] (weight == nullptr: 1), slots in order.  All K loads of U accesses are issued before
-// the first is used; K slots a round, and further rounds for k > K.
-template <typename T, int VB, int K, int U>
+// The rows of K slots of a token: pointers (nullptr: no row) and weights, in every lane of its warp
+template <typename V, int K> struct SlotRows {
+  const V* row[K];
+  float w[K];
+  __device__ __forceinline__ void get(const V* base, int mine, float my_w, int j0, int chunks) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      const int r = j0 + j < 32 ? __shfl_sync(0xffffffffu, mine, j0 + j) : -1;      // lanes beyond k hold -1
+      w[j] = __shfl_sync(0xffffffffu, my_w, (j0 + j) & 31);
+      row[j] = r >= 0 ? base + (int64_t)r * chunks : nullptr;
+    }
+  }
+};
+
+// out[t] = sum_j w[t,j] * ys[slot_row[t,j]] (weight == nullptr: 1), slots in order.  All loads of K slots and U accesses are issued
+// before the first is used; ONCE: the token's slots are one such round.
+template <typename T, int VB, int K, int U, bool ONCE>
 __global__ void __launch_bounds__(DW * 32)
 dispatch_combine_kernel(const T* __restrict__ ys, const void* __restrict__ weight, int w_bf16,
                         const int32_t* __restrict__ slot_row, int64_t n_tokens, int top_k, int chunks, int parts, int part,
@@ -348,35 +362,33 @@ dispatch_combine_kernel(const T* __restrict__ ys, const void* __restrict__ weigh
   const V* src = reinterpret_cast<const V*>(ys);
   V* dst = reinterpret_cast<V*>(out) + t * chunks;
   const int c_lo = parts == 1 ? 0 : (int)(wi % parts) * part * 32, c_hi = min(chunks, c_lo + part * 32);
+  SlotRows<V, K> rows;
+  if (ONCE) rows.get(src, mine, my_w, 0, chunks);
   for (int c0 = c_lo + lane; c0 - lane < c_hi; c0 += 32 * U) {
     float acc[U][X::N];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < X::N; ++i) acc[u][i] = 0.f;
-    for (int j0 = 0; j0 < top_k; j0 += K) {
+    for (int j0 = 0; j0 < (ONCE ? 1 : top_k); j0 += K) {
+      if (!ONCE) rows.get(src, mine, my_w, j0, chunks);
       V v[U][K];
-      int r[K];
 #pragma unroll
-      for (int j = 0; j < K; ++j) {
-        r[j] = j0 + j < 32 ? __shfl_sync(0xffffffffu, mine, j0 + j) : -1;       // lanes beyond k hold -1
-        const V* row = src + (int64_t)r[j] * chunks;
+      for (int j = 0; j < K; ++j)
+        if (rows.row[j] != nullptr)
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (r[j] >= 0 && c0 + u * 32 < c_hi) v[u][j] = __ldcs(row + c0 + u * 32);
-      }
+          for (int u = 0; u < U; ++u)
+            if (c0 + u * 32 < c_hi) v[u][j] = __ldcs(rows.row[j] + c0 + u * 32);
 #pragma unroll
-      for (int j = 0; j < K; ++j) {
-        const float w = __shfl_sync(0xffffffffu, my_w, (j0 + j) & 31);
+      for (int j = 0; j < K; ++j)
+        if (rows.row[j] != nullptr)
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (r[j] >= 0 && c0 + u * 32 < c_hi) {
+          for (int u = 0; u < U; ++u) {
             float f[X::N];
-            X::unpack(v[u][j], f);
+            X::unpack(v[u][j], f);             // beyond c_hi: whatever the register holds, not stored
 #pragma unroll
-            for (int i = 0; i < X::N; ++i) acc[u][i] = fmaf(f[i], w, acc[u][i]);
+            for (int i = 0; i < X::N; ++i) acc[u][i] = fmaf(f[i], rows.w[j], acc[u][i]);
           }
-      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -384,13 +396,13 @@ dispatch_combine_kernel(const T* __restrict__ ys, const void* __restrict__ weigh
   }
 }
 
-// dys rows and dw of a token's slots, WPT warps per token (1, or all DW for few tokens) that share its columns; blocks behind
-// the tokens' zero the rows of dys without a slot
-template <typename T, int VB, int K>
+// dys rows and dw of a token's slots, WPT warps per token (more for few tokens) that share its columns; blocks behind the tokens'
+// zero the rows of dys without a slot
+template <typename T, int VB, int K, int WPT>
 __global__ void __launch_bounds__(DW * 32)
 dispatch_combine_bwd_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __restrict__ ys,
                             const void* __restrict__ weight, int w_bf16, const int32_t* __restrict__ slot_row,
-                            const int32_t* __restrict__ row_slot, int64_t n_tokens, int top_k, int64_t rows, int chunks, int wpt,
+                            const int32_t* __restrict__ row_slot, int64_t n_tokens, int top_k, int64_t rows_, int chunks,
                             int64_t token_blocks, T* __restrict__ dys, void* __restrict__ dweight) {
   using V = typename RowVec<VB>::type;
   using X = RowElems<T, VB>;
@@ -398,10 +410,10 @@ dispatch_combine_bwd_kernel(const T* __restrict__ dout, int64_t dout_stride, con
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   V* dst = reinterpret_cast<V*>(dys);
   if ((int64_t)blockIdx.x >= token_blocks) {
-    zero_empty_rows<VB>(row_slot, (((int64_t)blockIdx.x - token_blocks) * DW + warp) * DZ_ROWS, rows, chunks, dst, lane);
+    zero_empty_rows<VB>(row_slot, (((int64_t)blockIdx.x - token_blocks) * DW + warp) * DZ_ROWS, rows_, chunks, dst, lane);
     return;
   }
-  const int64_t t = wpt == 1 ? (int64_t)blockIdx.x * DW + warp : blockIdx.x;
+  const int64_t t = (int64_t)blockIdx.x * (DW / WPT) + warp / WPT;
   const bool in = t < n_tokens;
   const V* g = reinterpret_cast<const V*>(dout + t * dout_stride);
   const V* src = reinterpret_cast<const V*>(ys);
@@ -411,24 +423,22 @@ dispatch_combine_bwd_kernel(const T* __restrict__ dout, int64_t dout_stride, con
   float my_dw = 0.f;
   if (__any_sync(0xffffffffu, mine >= 0)) {
     for (int j0 = 0; j0 < top_k; j0 += K) {
-      float dot[K], w[K];
-      int r[K];
+      SlotRows<V, K> rows;
+      rows.get(src, mine, my_w, j0, chunks);
+      float dot[K];
 #pragma unroll
-      for (int j = 0; j < K; ++j) {
-        dot[j] = 0.f;
-        r[j] = j0 + j < 32 ? __shfl_sync(0xffffffffu, mine, j0 + j) : -1;
-        w[j] = __shfl_sync(0xffffffffu, my_w, (j0 + j) & 31);
-      }
-      for (int c = (wpt == 1 ? 0 : warp * 32) + lane; c < chunks; c += 32 * wpt) {
-        V gv = g[c], v[K];
+      for (int j = 0; j < K; ++j) dot[j] = 0.f;
+      for (int c = (warp % WPT) * 32 + lane; c < chunks; c += 32 * WPT) {
+        const V gv = g[c];
+        V v[K];
 #pragma unroll
         for (int j = 0; j < K; ++j)
-          if (want && r[j] >= 0) v[j] = __ldcs(src + (int64_t)r[j] * chunks + c);
+          if (want && rows.row[j] != nullptr) v[j] = __ldcs(rows.row[j] + c);
         float gf[X::N];
         X::unpack(gv, gf);
 #pragma unroll
         for (int j = 0; j < K; ++j)
-          if (r[j] >= 0) {
+          if (rows.row[j] != nullptr) {
             float f[X::N];
             if (want) {
               X::unpack(v[j], f);
@@ -436,8 +446,8 @@ dispatch_combine_bwd_kernel(const T* __restrict__ dout, int64_t dout_stride, con
               for (int i = 0; i < X::N; ++i) dot[j] = fmaf(gf[i], f[i], dot[j]);
             }
 #pragma unroll
-            for (int i = 0; i < X::N; ++i) f[i] = gf[i] * w[j];
-            dst[(int64_t)r[j] * chunks + c] = X::pack(f);
+            for (int i = 0; i < X::N; ++i) f[i] = gf[i] * rows.w[j];
+            dst[rows.row[j] - src + c] = X::pack(f);
           }
       }
       if (want) {
@@ -451,13 +461,13 @@ dispatch_combine_bwd_kernel(const T* __restrict__ dout, int64_t dout_stride, con
     }
   }
   if (!want) return;
-  if (wpt > 1) {
+  if (WPT > 1) {
     red[warp][lane] = my_dw;
     __syncthreads();
-    if (warp != 0) return;
+    if (warp % WPT != 0) return;
     my_dw = 0.f;
 #pragma unroll
-    for (int i = 0; i < DW; ++i) my_dw += red[i][lane];
+    for (int i = 0; i < WPT; ++i) my_dw += red[warp + i][lane];
   }
   if (in && lane < top_k) {
     if (w_bf16) static_cast<__nv_bfloat16*>(dweight)[t * top_k + lane] = __float2bfloat16_rn(my_dw);
@@ -481,10 +491,11 @@ static int dispatch_check(const char* what, int64_t n_tokens, int hidden, int n_
   return BIBO_OK;
 }
 static unsigned dispatch_grid(int64_t warps) { return (unsigned)((warps + DW - 1) / DW); }
-// parts a row is cut into, and their size in accesses of a warp: enough warps for every SM to have 16, where the row allows it
+// parts a row is cut into, and their size in accesses of a warp: enough warps for every SM to have 64, where the row allows it
+// (5003 tokens x 3 slots x 1153 fp32 combine: 24.2 us with the 34 warps an SM that the tokens make)
 static int row_parts(int64_t n_tokens, int chunks, int* part) {
   const int steps = (chunks + 31) / 32;
-  const int64_t want = (16 * (int64_t)sm_count() + n_tokens - 1) / n_tokens;
+  const int64_t want = (64 * (int64_t)sm_count() + n_tokens - 1) / n_tokens;
   const int parts = want < steps ? (int)want : steps;
   *part = (steps + parts - 1) / parts;
   return (steps + *part - 1) / *part;
@@ -586,14 +597,16 @@ static void combine_v(const void* ys, const void* weight, int w_bf16, const int3
   int part;
   const int parts = row_parts(n_tokens, chunks, &part);
   const unsigned grid = dispatch_grid(n_tokens * parts);
-#define BIBO_COMBINE(K, U)                                                                                                  \
-  dispatch_combine_kernel<T, VB, K, U><<<grid, DW * 32, 0, st>>>(static_cast<const T*>(ys), weight, w_bf16, slot_row, n_tokens, \
+#define BIBO_COMBINE(K, U, ONCE)                                                                                            \
+  dispatch_combine_kernel<T, VB, K, U, ONCE><<<grid, DW * 32, 0, st>>>(static_cast<const T*>(ys), weight, w_bf16, slot_row, n_tokens, \
                                                                  top_k, chunks, parts, part, static_cast<T*>(out))
-  if (top_k == 1) BIBO_COMBINE(1, 4);
-  else if (top_k == 2) BIBO_COMBINE(2, 4);
-  else if (top_k <= 4) BIBO_COMBINE(4, 2);
-  else if (top_k <= 6) BIBO_COMBINE(6, 2);
-  else BIBO_COMBINE(8, 2);
+  constexpr int M = VB == 16 ? 1 : 2;            // narrow accesses: more of them in flight
+  if (top_k == 1) BIBO_COMBINE(1, 4 * M, true);
+  else if (top_k == 2) BIBO_COMBINE(2, 4 * M, true);
+  else if (top_k <= 4) BIBO_COMBINE(4, 2 * M, true);
+  else if (top_k <= 6) BIBO_COMBINE(6, 2 * M, true);
+  else if (top_k <= 8) BIBO_COMBINE(8, 2 * M, true);
+  else BIBO_COMBINE(8, 2 * M, false);
 #undef BIBO_COMBINE
 }
 template <typename T>
@@ -629,19 +642,28 @@ static void combine_bwd_v(const void* dout, int64_t dout_stride, const void* ys,
                           const int32_t* slot_row, const int32_t* row_slot, int64_t n_tokens, int top_k, int64_t rows, int hidden,
                           void* dys, void* dweight, cudaStream_t st) {
   const int chunks = hidden / RowElems<T, VB>::N;
-  const int wpt = n_tokens < 4 * (int64_t)sm_count() ? DW : 1;      // a block per token where warps per token would be few
-  const int64_t token_blocks = wpt == 1 ? (n_tokens + DW - 1) / DW : n_tokens;
+  // warps per token: enough for 32 an SM
+  const int64_t want = 32 * (int64_t)sm_count();
+  const int wpt = n_tokens >= want ? 1 : 4 * n_tokens >= want ? 4 : DW;
+  const int64_t token_blocks = (n_tokens * wpt + DW - 1) / DW;
   const unsigned grid = (unsigned)token_blocks + dispatch_grid((rows + DZ_ROWS - 1) / DZ_ROWS);
-#define BIBO_COMBINE(K)                                                                                                      \
-  dispatch_combine_bwd_kernel<T, VB, K><<<grid, DW * 32, 0, st>>>(static_cast<const T*>(dout), dout_stride,                  \
-                                                                  static_cast<const T*>(ys), weight, w_bf16, slot_row,       \
-                                                                  row_slot, n_tokens, top_k, rows, chunks, wpt, token_blocks, \
-                                                                  static_cast<T*>(dys), dweight)
+#define BIBO_COMBINE_W(K, WPT)                                                                                               \
+  dispatch_combine_bwd_kernel<T, VB, K, WPT><<<grid, DW * 32, 0, st>>>(static_cast<const T*>(dout), dout_stride,             \
+                                                                       static_cast<const T*>(ys), weight, w_bf16, slot_row,  \
+                                                                       row_slot, n_tokens, top_k, rows, chunks, token_blocks, \
+                                                                       static_cast<T*>(dys), dweight)
+#define BIBO_COMBINE(K)                      \
+  do {                                       \
+    if (wpt == 1) BIBO_COMBINE_W(K, 1);      \
+    else if (wpt == 4) BIBO_COMBINE_W(K, 4); \
+    else BIBO_COMBINE_W(K, DW);              \
+  } while (0)
   if (top_k == 1) BIBO_COMBINE(1);
   else if (top_k == 2) BIBO_COMBINE(2);
   else if (top_k <= 4) BIBO_COMBINE(4);
   else if (top_k <= 6) BIBO_COMBINE(6);
   else BIBO_COMBINE(8);
+#undef BIBO_COMBINE_W
 #undef BIBO_COMBINE
 }
 template <typename T>
