@@ -81,6 +81,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 __device__ __forceinline__ void fence_barrier_init() {
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
+// orders this thread's writes to any CTA's shared memory before later asynchronous reads of them
+__device__ __forceinline__ void fence_proxy_async_all() { asm volatile("fence.proxy.async;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -160,6 +162,19 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
       : "r"(taddr)
       : "memory");
 }
+// ... and back
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+      "%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Instruction descriptor: bf16 x bf16 -> fp32, both operands K-major, M x N tile.
@@ -266,9 +281,9 @@ constexpr int EPI_THREADS = 128;
 // Shared-memory matrix descriptor for an MN-major operand staged as boxes of [64 k-rows x 64 elements (128 bytes)]
 // written by TMA with the 128-byte swizzle (see gemm_bwd_tc.cu).
 constexpr int MN_BOX = 64 * BK * 2;   // one [64 k-rows x 128 B] box
-__device__ __forceinline__ uint64_t make_sdesc_mn128(uint32_t smem_addr) {
+__device__ __forceinline__ uint64_t make_sdesc_mn128(uint32_t smem_addr, uint32_t box_bytes = MN_BOX) {
   uint64_t d = (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)(MN_BOX >> 4) << 16;   // leading byte offset: next 64 elements along M/N
+  d |= (uint64_t)(box_bytes >> 4) << 16;   // leading byte offset: next 64 elements along M/N
   d |= (uint64_t)(1024 >> 4) << 32;     // stride byte offset: next 8 k-rows
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;

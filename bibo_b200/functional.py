@@ -702,7 +702,8 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHU
     if update.numel() == 0:
         return out
     lib = _lib.load()
-    ws = torch.empty(int(lib.bibo_moe_orthogonalize_workspace(batch, m, n)), dtype=torch.uint8, device=update.device)
+    words = int(lib.bibo_moe_orthogonalize_workspace(batch, m, n))
+    ws = torch.empty(words, dtype=torch.uint8, device=update.device) if words else None
     flat = (C.c_float * (3 * steps))(*[float(v) for c in co for v in c])
     p = _lib.ptr
     _launch("bibo_moe_orthogonalize", update.device, p(u), batch, u.stride(0), m, n, u.stride(1), dt, steps,

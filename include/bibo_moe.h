@@ -599,7 +599,7 @@ int bibo_moe_dispatch_combine_bwd(const void* dout, int64_t dout_stride, const v
  * coefficients_host[3 * step ..]; out [batch, rows, cols] is bfloat16 and contiguous.  f16 operands, fp32 accumulation;
  * the polynomials must keep the singular values below 4 (|b G + c G^2| below 16).  |u|_F^2 is summed in fp32.
  * workspace: bibo_moe_orthogonalize_workspace bytes, 128-byte aligned (2 GiB at most, more only where one
- * matrix needs it).  If a bounded wait gives up, the whole result of its group of matrices is NaN.   */
+ * matrix needs it; 0, and NULL, where the matrices are small enough for shared memory).  If a bounded wait gives up, the whole result of its group of matrices is NaN.   */
 int64_t bibo_moe_orthogonalize_workspace(int64_t batch, int rows, int cols);
 int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batch_stride, int rows, int cols, int64_t row_stride,
                            int dtype, int steps, const float* coefficients_host, float eps, void* workspace, void* out,

@@ -91,7 +91,8 @@ def _momentum(shape, dtype, seed, rank=8, floor=0.1, scale=1e-3):
 
 
 SHAPES = [(1, 1), (1, 7), (5, 1), (2, 3), (64, 64), (64, 2048), (2048, 64), (128, 128), (127, 129), (130, 257), (200, 72),
-          (3, 65, 300), (2, 3, 100, 40), (4, 256, 512), (5, 512, 128), (2, 300, 900), (1, 640, 640), (2, 1030, 777)]
+          (3, 65, 300), (2, 3, 100, 40), (4, 256, 512), (5, 512, 128), (2, 300, 900), (1, 640, 640), (2, 1030, 777),
+          (100, 384), (100, 385), (20, 100, 500), (128, 1536), (1537, 96), (7, 3000), (2500, 128), (150, 33, 129)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -153,13 +154,20 @@ def test_zero_matrices_and_empty_stacks():
 
 
 def test_many_matrices():
-    """More matrices than one group of the workspace holds."""
+    """Many small ones, and more larger ones than a workspace holds at once."""
+    from bibo_b200 import _lib
     from bibo_b200 import functional as Fn
     u = _momentum((33000, 8, 16), torch.bfloat16, 2)
     got = Fn.orthogonalize(u)
     for i in (0, 1, 16383, 16384, 32767, 32768, 32999):
         assert torch.equal(got[i], Fn.orthogonalize(u[i]))
     _check(u[32760:32776].clone())
+    size = _lib.load().bibo_moe_orthogonalize_workspace
+    assert size(320, 640, 1024) == size(10000, 640, 1024) > 1 << 30       # a group of fewer than 320
+    u = _momentum((320, 640, 1024), torch.bfloat16, 3)
+    got = Fn.orthogonalize(u)
+    for i in (0, 150, 297, 298, 299, 300, 319):
+        assert torch.equal(got[i], Fn.orthogonalize(u[i]))
 
 
 def test_two_graphs_and_streams_do_not_share_a_workspace():

@@ -151,16 +151,17 @@ def test_orthogonalize_refusals_and_workspace():
     lib, p = _lib.load(), _dummy()
     co = (ctypes.c_float * 3)(1.5, -0.5, 0.0)
     aligned = (p + 127) & ~127
-    call = lambda batch=2, bs=64 * 32, r=64, c=32, rs=32, dt=_lib.F32, steps=1, u=p, ws=aligned, out=p: lib.bibo_moe_orthogonalize(
+    call = lambda batch=2, bs=640 * 320, r=640, c=320, rs=320, dt=_lib.F32, steps=1, u=p, ws=aligned, out=p: lib.bibo_moe_orthogonalize(
         u, batch, bs, r, c, rs, dt, steps, co, 1e-7, ws, out, None)
     err = lambda: lib.bibo_moe_last_error_string()
     assert call(dt=3) == -1 and call(steps=0) == -1 and call(steps=65) == -1 and b"steps=65" in err()
-    assert call(rs=31) == -1 and call(bs=64 * 32 - 1) == -1 and b"overlapping" in err()
+    assert call(rs=319) == -1 and call(bs=640 * 320 - 1) == -1 and b"overlapping" in err()
     assert call(u=None) == -1 and call(ws=None) == -1 and call(out=None) == -1
     assert call(ws=aligned + 16) == -2 and call(r=-1) == -1
     assert call(batch=0) == 0 and call(r=0) == 0
     size = lib.bibo_moe_orthogonalize_workspace
-    assert size(0, 5, 5) == 0 and size(64, 1024, 2048) == size(64, 2048, 1024) <= 1 << 31
+    assert size(0, 5, 5) == 0 and size(7, 128, 300) == size(7, 300, 128) == 0 and size(7, 129, 300) > 0
+    assert size(64, 1024, 2048) == size(64, 2048, 1024) <= 1 << 31
     assert size(10000, 1024, 2048) <= 1 << 31 and size(1, 20000, 20000) > 1 << 31
     fake = lambda *s, **k: _fake(torch.zeros(*s, **k))
     with pytest.raises(RuntimeError, match="no CPU implementation"):
