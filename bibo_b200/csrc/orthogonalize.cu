@@ -23,6 +23,7 @@
 // Symmetric products (G, F, T, R, the second G) are computed and stored on and below the diagonal's 256 x 256 tiles only; an
 // operand tile above it is read as the transposed tile below it, as an MN-major operand.
 #include <algorithm>
+#include <type_traits>
 #include <cuda_fp16.h>
 
 #include "tc_common.cuh"
@@ -32,18 +33,19 @@ namespace tc {
 
 constexpr float NS_ONE = 4096.f;                 // 1.0 as stored
 constexpr float NS_LO = 2048.f;                  // scale of the lower half of a value beside the upper one
-constexpr int NS_MAX_PARTS = 64;                 // partial sums of squares per matrix
+constexpr int NS_MAX_PARTS = 256;                // partial sums of squares per matrix
 
 // ---- products ----------------------------------------------------------------------------------------------------
-// One persistent kernel on 256 x 256 tiles: a CTA pair runs tcgen05.mma.cta_group::2 (256 x 256 x 16), each CTA staging its 128
-// rows of A and its half of B's rows, five stages of 32 KB; 2 x 256 TMEM columns, so the drain of a tile runs under the next
-// one's products.  Warps: 0 loads, 1 products (pair leader), 2 loads the sources of the drain and stores its results,
-// 4-7 drain.  Sub-tiles of 64 columns go through two 32 KB slots: source halves in, result halves out, in place.
+// 256 x 256 tiles: a CTA pair runs tcgen05.mma.cta_group::2 (256 x 256 x 16), each CTA staging its 128 rows of A and its half of
+// B's rows, five stages of 32 KB.  Warps: 0 loads, 1 products (pair leader), 2 loads the sources of the drain and stores its
+// results, 4-11 drain (two warps per quarter of the rows, 32 columns each: with one, a scheduler has nothing to run while its
+// warp waits, and a sub-tile took 1600 cycles).  Results leave in sub-tiles of 64 columns through slots of 16 KB (32 KB where
+// values come or go in two halves): source halves in, result halves out, in place.
 constexpr int NS_GRAM = 0, NS_SYM = 1, NS_APPLY = 2;
-constexpr int NS_T = 256, NS_STAGES = 5, NS_THREADS = 256;
+constexpr int NS_T = 256, NS_STAGES = 5, NS_DRAIN = 256, NS_THREADS = 128 + NS_DRAIN;
 constexpr int NS_OFF_A = 0;
 constexpr int NS_OFF_B = NS_OFF_A + NS_STAGES * A_BYTES;
-constexpr int NS_OFF_SLOT = NS_OFF_B + NS_STAGES * A_BYTES;      // [2] slots of {upper [128 x 64], lower [128 x 64]}
+constexpr int NS_OFF_SLOT = NS_OFF_B + NS_STAGES * A_BYTES;      // 4 slots of {upper [128 x 64]} or 2 of {upper, lower}
 constexpr int NS_OFF_BAR = NS_OFF_SLOT + 4 * C_SUB;
 constexpr int NS_SMEM = NS_OFF_BAR + 256 + 1024;
 
@@ -109,92 +111,204 @@ __device__ __forceinline__ void ns_load(unsigned char* dst, const NsMaps& m, uin
   }
 }
 
+template <int MODE, bool TALL> struct NsOps {
+  static constexpr int A = MODE == NS_GRAM ? (TALL ? OP_MN : OP_K) : MODE == NS_SYM ? OP_SYM : TALL ? OP_K : OP_SYM;
+  static constexpr int B = MODE == NS_GRAM ? (TALL ? OP_MN : OP_K) : MODE == NS_SYM ? OP_SYM : TALL ? OP_SYM : OP_MN;
+  // both operands of a CTA are the same rows of x
+  static __device__ __forceinline__ bool same(const NsTile& t) { return MODE == NS_GRAM && t.i == t.j; }
+};
+
+struct NsBars {                                  // barriers and flags in shared memory
+  uint64_t *full, *empty, *tfull, *tempty, *sfull, *cfull, *pfull;   // [stages], [stages], [2], [2], [4], [4], [1]
+  uint32_t* tmem_slot;
+  volatile int* abort_flag;
+  __device__ explicit NsBars(unsigned char* smem) {
+    full = reinterpret_cast<uint64_t*>(smem + NS_OFF_BAR);   // pair leader
+    empty = full + NS_STAGES;
+    tfull = empty + NS_STAGES;
+    tempty = tfull + 2;                                      // pair leader: the drain warps of both CTAs
+    sfull = tempty + 2;                                      // a slot's sources have landed (and its last store has left)
+    cfull = sfull + 4;                                       // a slot's results are written
+    pfull = cfull + 4;                                       // the other pairs' partial sums have landed
+    tmem_slot = reinterpret_cast<uint32_t*>(pfull + 1);
+    abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  }
+  __device__ __forceinline__ void init() const {
+    for (int s = 0; s < NS_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 2 * NS_DRAIN / 32); }
+    for (int b = 0; b < 4; ++b) { mbar_init(&sfull[b], 1); mbar_init(&cfull[b], NS_DRAIN); }
+    mbar_init(pfull, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+};
+
+// k-blocks [k0, k1) of a tile into the stages; one thread of each CTA of the pair
+template <int MODE, bool TALL, int STAGES = NS_STAGES>
+__device__ __forceinline__ bool ns_produce(unsigned char* smem, const NsArgs& p, const NsBars& s, const NsTile& t, int k0, int k1,
+                                           int pr, uint32_t leader, PipeState& ps) {
+  using Ops = NsOps<MODE, TALL>;
+  const bool same = Ops::same(t);
+  for (int kb = k0; kb < k1; ++kb) {
+    if (!mbar_wait<true>(&s.empty[ps.stage], ps.phase ^ 1, s.abort_flag)) return false;
+    if (pr == 0) mbar_expect_tx(&s.full[ps.stage], same ? 2 * A_BYTES : 4 * A_BYTES);
+    const uint32_t bar = map_to_cta(&s.full[ps.stage], leader);
+    ns_load<Ops::A>(smem + NS_OFF_A + ps.stage * A_BYTES, p.a, bar, t.i, pr, kb, t.b);
+    if (!same) ns_load<Ops::B>(smem + NS_OFF_A + (STAGES + ps.stage) * A_BYTES, p.b, bar, t.j, pr, kb, t.b);
+    ps.next<STAGES>();
+  }
+  return true;
+}
+// ... and their products onto 256 accumulator columns; one thread of the pair leader
+template <int MODE, bool TALL, int STAGES = NS_STAGES>
+__device__ __forceinline__ bool ns_multiply(unsigned char* smem, const NsBars& s, const NsTile& t, int k0, int k1, uint32_t tmem_d,
+                                            uint16_t pair_mask, PipeState& ps) {
+  using Ops = NsOps<MODE, TALL>;
+  const bool same = Ops::same(t);
+  for (int kb = k0; kb < k1; ++kb) {
+    if (!mbar_wait<true>(&s.full[ps.stage], ps.phase, s.abort_flag)) return false;
+    tc_fence_after();
+    const uint32_t sa = smem_u32(smem + NS_OFF_A + ps.stage * A_BYTES);
+    const uint32_t sb = same ? sa : smem_u32(smem + NS_OFF_A + (STAGES + ps.stage) * A_BYTES);
+    const bool amn = ns_mn_major<Ops::A>(t.i, kb), bmn = ns_mn_major<Ops::B>(t.j, kb);
+    const uint64_t da = amn ? make_sdesc_mn128(sa) : make_sdesc_k128(sa);
+    const uint64_t db = bmn ? make_sdesc_mn128(sb) : make_sdesc_k128(sb);
+    const int a_step = amn ? (2048 >> 4) : (32 >> 4), b_step = bmn ? (2048 >> 4) : (32 >> 4);
+    // bit 15: A is MN-major, bit 16: B is MN-major
+    const uint32_t idesc = make_idesc_f16(2 * BM, NS_T) | (amn ? 1u << 15 : 0u) | (bmn ? 1u << 16 : 0u);
+#pragma unroll
+    for (int k = 0; k < BK / UK; ++k)
+      umma_bf16_cg2(tmem_d, da + k * a_step, db + k * b_step, idesc, (kb > k0) | (k != 0));
+    umma_commit_cg2_mc(&s.empty[ps.stage], pair_mask);
+    ps.next<STAGES>();
+  }
+  return true;
+}
+
+struct NsScale { float al, be, bl; bool poison; };
+template <int MODE> __device__ __forceinline__ NsScale ns_scale(const NsArgs& p, int b, bool poison) {
+  NsScale c{p.alpha, p.beta, p.beta_lo, poison};
+  if (p.t_scale != nullptr) {
+    const float ts = p.t_scale[b];
+    c.al *= MODE == NS_GRAM ? ts * ts : ts;
+    c.be *= ts;
+    c.bl *= ts;
+  }
+  return c;
+}
+// 32 accumulator columns of a row (half `h` of a sub-tile) and its sources -> results, in the slot
+__device__ __forceinline__ void ns_finish(const NsArgs& p, const NsScale& c, const float (&acc)[32], unsigned char* slot, int row,
+                                          int h) {
+#pragma unroll
+  for (int jj = 0; jj < 4; ++jj) {
+    uint4* hi = reinterpret_cast<uint4*>(slot + swz(row, 4 * h + jj));
+    uint4* lo = reinterpret_cast<uint4*>(slot + C_SUB + swz(row, 4 * h + jj));
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c.al * acc[8 * jj + i];
+    if (p.has_s) {
+      const uint4 s = *hi;
+      const uint32_t* ps = reinterpret_cast<const uint32_t*>(&s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack_f16(ps[i]);
+        v[2 * i] = fmaf(c.be, f.x, v[2 * i]);
+        v[2 * i + 1] = fmaf(c.be, f.y, v[2 * i + 1]);
+      }
+    }
+    if (p.has_lo) {
+      const uint4 s = *lo;
+      const uint32_t* ps = reinterpret_cast<const uint32_t*>(&s);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack_f16(ps[i]);
+        v[2 * i] = fmaf(c.bl, f.x, v[2 * i]);
+        v[2 * i + 1] = fmaf(c.bl, f.y, v[2 * i + 1]);
+      }
+    }
+    uint4 o;
+    uint32_t* po = reinterpret_cast<uint32_t*>(&o);
+    if (p.out_bf16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        po[i] = c.poison ? 0x7fff7fffu : pack_bf16(v[2 * i] * (1.f / NS_ONE), v[2 * i + 1] * (1.f / NS_ONE));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) po[i] = pack_f16(v[2 * i], v[2 * i + 1]);
+    }
+    *hi = o;
+    if (p.out_lo) {
+      uint4 l;
+      uint32_t* pl = reinterpret_cast<uint32_t*>(&l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack_f16(po[i]);
+        pl[i] = pack_f16((v[2 * i] - f.x) * NS_LO, (v[2 * i + 1] - f.y) * NS_LO);
+      }
+      *lo = l;
+    }
+  }
+}
+// a wait gave up: lets copies in flight to this shared memory end, raises the status and voids this CTA's part of the caller's result
+template <int MODE> __device__ __forceinline__ void ns_give_up(const NsArgs& p, int64_t w0, int64_t dw, int pr) {
+  for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+  if (threadIdx.x == 0) atomicExch(p.status, 112);
+  if (!p.out_bf16) return;
+  for (int64_t w = w0; w < p.n_work; w += dw) {
+    const NsTile t = ns_decode<MODE>(w, p.m_tiles, p.n_tiles);
+    for (int i = threadIdx.x; i < BM * NS_T; i += NS_THREADS) {
+      const int y = t.i * NS_T + pr * BM + i / NS_T, x = t.j * NS_T + i % NS_T;
+      if (y < p.rows && x < p.cols) p.out[((int64_t)t.b * p.rows + y) * p.cols + x] = __ushort_as_bfloat16(0x7fff);
+    }
+  }
+}
+__device__ __forceinline__ unsigned char* ns_smem() {
+  extern __shared__ unsigned char smem_dyn[];
+  return reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+}
+
+// Many tiles: persistent pairs, 2 x 256 accumulator columns, so the drain of a tile runs under the next one's products.
 template <int MODE, bool TALL>
 __global__ void __launch_bounds__(NS_THREADS, 1)
 ns_product_kernel(const __grid_constant__ NsArgs p) {
-  constexpr int OP_A = MODE == NS_GRAM ? (TALL ? OP_MN : OP_K) : MODE == NS_SYM ? OP_SYM : TALL ? OP_K : OP_SYM;
-  constexpr int OP_B = MODE == NS_GRAM ? (TALL ? OP_MN : OP_K) : MODE == NS_SYM ? OP_SYM : TALL ? OP_SYM : OP_MN;
-  extern __shared__ unsigned char smem_dyn[];
-  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + NS_OFF_BAR);   // pair leader
-  uint64_t* empty = full + NS_STAGES;
-  uint64_t* tfull = empty + NS_STAGES;
-  uint64_t* tempty = tfull + 2;                                      // pair leader: 4 drain warps of each CTA
-  uint64_t* sfull = tempty + 2;                                      // a slot's sources have landed (and its last store has left)
-  uint64_t* cfull = sfull + 2;                                       // a slot's results are written
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cfull + 2);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  unsigned char* smem = ns_smem();
+  const NsBars s(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pr = (int)(cluster_ctarank() & 1u);
   const int64_t w0 = blockIdx.x / 2, dw = gridDim.x / 2;
+  pdl_launch_next();
   if (threadIdx.x == 0) {
-    for (int s = 0; s < NS_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 8);
-      mbar_init(&sfull[b], 1); mbar_init(&cfull[b], EPI_THREADS);
-    }
-    *abort_flag = 0;
-    fence_barrier_init();
+    s.init();
     prefetch_tmap(&p.a.r128); prefetch_tmap(&p.a.r64); prefetch_tmap(&p.b.r128); prefetch_tmap(&p.b.r64);
     prefetch_tmap(&p.s_hi); prefetch_tmap(&p.c_hi);
   }
-  if (warp == 1) { tmem_alloc_cg2(tmem_slot, 2 * NS_T); tmem_relinquish_cg2(); }
+  if (warp == 1) { tmem_alloc_cg2(s.tmem_slot, 2 * NS_T); tmem_relinquish_cg2(); }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = *s.tmem_slot;
+  pdl_wait();
+  const int halves = p.has_lo || p.out_lo ? 2 : 1, slots = 4 / halves, slot_bits = slots == 4 ? 2 : 1;
+  auto slot_at = [&](int64_t u) { return smem + NS_OFF_SLOT + (int)(u & (slots - 1)) * halves * C_SUB; };
 
   if (warp == 0) {
     if (elect_one()) {
       PipeState ps;
       bool ok = true;
-      for (int64_t w = w0; w < p.n_work && ok; w += dw) {
-        const NsTile t = ns_decode<MODE>(w, p.m_tiles, p.n_tiles);
-        const bool same = MODE == NS_GRAM && t.i == t.j;             // both operands of a CTA are the same rows
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
-          ok = mbar_wait<true>(&empty[ps.stage], ps.phase ^ 1, abort_flag);
-          if (!ok) break;
-          if (pr == 0) mbar_expect_tx(&full[ps.stage], same ? 2 * A_BYTES : 4 * A_BYTES);
-          const uint32_t bar = map_to_cta(&full[ps.stage], 0);
-          ns_load<OP_A>(smem + NS_OFF_A + ps.stage * A_BYTES, p.a, bar, t.i, pr, kb, t.b);
-          if (!same) ns_load<OP_B>(smem + NS_OFF_B + ps.stage * A_BYTES, p.b, bar, t.j, pr, kb, t.b);
-          ps.next<NS_STAGES>();
-        }
-      }
+      for (int64_t w = w0; w < p.n_work && ok; w += dw)
+        ok = ns_produce<MODE, TALL>(smem, p, s, ns_decode<MODE>(w, p.m_tiles, p.n_tiles), 0, p.k_blocks, pr, 0, ps);
     }
   } else if (warp == 1) {
     if (pr == 0 && elect_one()) {
       PipeState ps;
       int acc = 0;
       uint32_t acc_phase = 0;
-      bool ok = true;
-      for (int64_t w = w0; w < p.n_work && ok; w += dw) {
-        const NsTile t = ns_decode<MODE>(w, p.m_tiles, p.n_tiles);
-        const bool same = MODE == NS_GRAM && t.i == t.j;
-        ok = mbar_wait<true>(&tempty[acc], acc_phase ^ 1, abort_flag);
-        if (!ok) break;
+      for (int64_t w = w0; w < p.n_work; w += dw) {
+        if (!mbar_wait<true>(&s.tempty[acc], acc_phase ^ 1, s.abort_flag)) break;
         tc_fence_after();
-        for (int kb = 0; kb < p.k_blocks; ++kb) {
-          ok = mbar_wait<true>(&full[ps.stage], ps.phase, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t sa = smem_u32(smem + NS_OFF_A + ps.stage * A_BYTES);
-          const uint32_t sb = same ? sa : smem_u32(smem + NS_OFF_B + ps.stage * A_BYTES);
-          const bool amn = ns_mn_major<OP_A>(t.i, kb), bmn = ns_mn_major<OP_B>(t.j, kb);
-          const uint64_t da = amn ? make_sdesc_mn128(sa) : make_sdesc_k128(sa);
-          const uint64_t db = bmn ? make_sdesc_mn128(sb) : make_sdesc_k128(sb);
-          const int a_step = amn ? (2048 >> 4) : (32 >> 4), b_step = bmn ? (2048 >> 4) : (32 >> 4);
-          // bit 15: A is MN-major, bit 16: B is MN-major
-          const uint32_t idesc = make_idesc_f16(2 * BM, NS_T) | (amn ? 1u << 15 : 0u) | (bmn ? 1u << 16 : 0u);
-#pragma unroll
-          for (int k = 0; k < BK / UK; ++k)
-            umma_bf16_cg2(tmem_base + acc * NS_T, da + k * a_step, db + k * b_step, idesc, (kb | k) != 0);
-          umma_commit_cg2_mc(&empty[ps.stage], 3);
-          ps.next<NS_STAGES>();
-        }
-        if (!ok) break;
-        umma_commit_cg2_mc(&tfull[acc], 3);
+        if (!ns_multiply<MODE, TALL>(smem, s, ns_decode<MODE>(w, p.m_tiles, p.n_tiles), 0, p.k_blocks, tmem_base + acc * NS_T, 3, ps)) break;
+        umma_commit_cg2_mc(&s.tfull[acc], 3);
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
       }
@@ -211,36 +325,34 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
       };
       auto source = [&](int64_t u) {
         if (u >= n_sub) return;
-        uint64_t* bar = &sfull[u & 1];
+        uint64_t* bar = &s.sfull[u & (slots - 1)];
         NsTile t;
         int x, y;
-        if (!place(u, t, x, y) || !p.has_s) { mbar_arrive(bar); return; }
-        unsigned char* slot = smem + NS_OFF_SLOT + (u & 1) * 2 * C_SUB;
+        if (!p.has_s || !place(u, t, x, y)) { mbar_arrive(bar); return; }
         mbar_expect_tx(bar, p.has_lo ? 2 * C_SUB : C_SUB);
-        tma_load_3d(slot, &p.s_hi, bar, x, y, t.b);
-        if (p.has_lo) tma_load_3d(slot + C_SUB, &p.s_lo, bar, x, y, t.b);
+        tma_load_3d(slot_at(u), &p.s_hi, bar, x, y, t.b);
+        if (p.has_lo) tma_load_3d(slot_at(u) + C_SUB, &p.s_lo, bar, x, y, t.b);
       };
-      source(0);
-      source(1);
+      for (int u = 0; u < slots; ++u) source(u);
       for (int64_t u = 0; u < n_sub; ++u) {
-        if (!mbar_wait(&cfull[u & 1], (uint32_t)(u >> 1) & 1u, abort_flag)) break;
+        if (!mbar_wait(&s.cfull[u & (slots - 1)], (uint32_t)(u >> slot_bits) & 1u, s.abort_flag)) break;
         NsTile t;
         int x, y;
         if (place(u, t, x, y)) {
-          unsigned char* slot = smem + NS_OFF_SLOT + (u & 1) * 2 * C_SUB;
-          tma_store_3d(&p.c_hi, slot, x, y, t.b);
-          if (p.out_lo) tma_store_3d(&p.c_lo, slot + C_SUB, x, y, t.b);
+          tma_store_3d(&p.c_hi, slot_at(u), x, y, t.b);
+          if (p.out_lo) tma_store_3d(&p.c_lo, slot_at(u) + C_SUB, x, y, t.b);
           tma_store_commit();
         }
-        if (u + 2 < n_sub) {
+        if (u + slots < n_sub) {
           tma_store_wait_read();
-          source(u + 2);
+          source(u + slots);
         }
       }
       tma_store_wait_all();
     }
   } else if (warp >= 4) {
     const int row = (warp & 3) * 32 + lane;
+    const int h = (warp - 4) >> 2;
     const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
     const bool poison = p.out_bf16 && *p.status != 0;                 // an earlier product gave up: no number is left to stand
     int acc = 0;
@@ -248,82 +360,27 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
     int64_t u = 0;
     bool ok = true;
     for (int64_t w = w0; w < p.n_work && ok; w += dw) {
-      float al = p.alpha, be = p.beta, bl = p.beta_lo;
-      if (p.t_scale != nullptr) {
-        const float ts = p.t_scale[ns_decode<MODE>(w, p.m_tiles, p.n_tiles).b];
-        al *= MODE == NS_GRAM ? ts * ts : ts;
-        be *= ts;
-        bl *= ts;
-      }
-      ok = mbar_wait<true>(&tfull[acc], acc_phase, abort_flag);
+      const NsScale c = ns_scale<MODE>(p, ns_decode<MODE>(w, p.m_tiles, p.n_tiles).b, poison);
+      ok = mbar_wait<true>(&s.tfull[acc], acc_phase, s.abort_flag);
       if (!ok) break;
+      __syncwarp();
       tc_fence_after();
 #pragma unroll 1
       for (int g = 0; g < 4; ++g, ++u) {
-        uint32_t r[2][32];
-        tmem_ld32(lane_addr + acc * NS_T + g * 64, r[0]);
-        tmem_ld32(lane_addr + acc * NS_T + g * 64 + 32, r[1]);
-        ok = mbar_wait(&sfull[u & 1], (uint32_t)(u >> 1) & 1u, abort_flag);
+        float r[32];
+        tmem_ld32(lane_addr + acc * NS_T + g * 64 + h * 32, reinterpret_cast<uint32_t*>(r));
+        ok = mbar_wait(&s.sfull[u & (slots - 1)], (uint32_t)(u >> slot_bits) & 1u, s.abort_flag);
+        __syncwarp();
         tmem_ld_wait();
         if (g == 3) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_addr(map_to_cta(&tempty[acc], 0));
+          if (lane == 0) mbar_arrive_cluster_addr(map_to_cta(&s.tempty[acc], 0));
         }
         if (!ok) break;
-        unsigned char* slot = smem + NS_OFF_SLOT + (u & 1) * 2 * C_SUB;
-#pragma unroll
-        for (int jj = 0; jj < 8; ++jj) {
-          uint4* hi = reinterpret_cast<uint4*>(slot + swz(row, jj));
-          uint4* lo = reinterpret_cast<uint4*>(slot + C_SUB + swz(row, jj));
-          const uint32_t* a = r[jj >> 2] + 8 * (jj & 3);
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = al * __uint_as_float(a[i]);
-          if (p.has_s) {
-            const uint4 s = *hi;
-            const uint32_t* ps = reinterpret_cast<const uint32_t*>(&s);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 f = unpack_f16(ps[i]);
-              v[2 * i] = fmaf(be, f.x, v[2 * i]);
-              v[2 * i + 1] = fmaf(be, f.y, v[2 * i + 1]);
-            }
-          }
-          if (p.has_lo) {
-            const uint4 s = *lo;
-            const uint32_t* ps = reinterpret_cast<const uint32_t*>(&s);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 f = unpack_f16(ps[i]);
-              v[2 * i] = fmaf(bl, f.x, v[2 * i]);
-              v[2 * i + 1] = fmaf(bl, f.y, v[2 * i + 1]);
-            }
-          }
-          uint4 o;
-          uint32_t* po = reinterpret_cast<uint32_t*>(&o);
-          if (p.out_bf16) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              po[i] = poison ? 0x7fff7fffu : pack_bf16(v[2 * i] * (1.f / NS_ONE), v[2 * i + 1] * (1.f / NS_ONE));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) po[i] = pack_f16(v[2 * i], v[2 * i + 1]);
-          }
-          *hi = o;
-          if (p.out_lo) {
-            uint4 l;
-            uint32_t* pl = reinterpret_cast<uint32_t*>(&l);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 f = unpack_f16(po[i]);
-              pl[i] = pack_f16((v[2 * i] - f.x) * NS_LO, (v[2 * i + 1] - f.y) * NS_LO);
-            }
-            *lo = l;
-          }
-        }
+        ns_finish(p, c, r, slot_at(u), row, h);
         fence_proxy_async_smem();
-        mbar_arrive(&cfull[u & 1]);
+        mbar_arrive(&s.cfull[u & (slots - 1)]);
       }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
@@ -332,21 +389,156 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (*abort_flag) {                             // a wait gave up: copies may still be in flight to this shared memory
-    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
-    if (threadIdx.x == 0) atomicExch(p.status, 112);
-    if (p.out_bf16) {                            // its part of the caller's result is void
-      for (int64_t w = w0; w < p.n_work; w += dw) {
-        const NsTile t = ns_decode<MODE>(w, p.m_tiles, p.n_tiles);
-        for (int i = threadIdx.x; i < BM * NS_T; i += NS_THREADS) {
-          const int y = t.i * NS_T + pr * BM + i / NS_T, x = t.j * NS_T + i % NS_T;
-          if (y < p.rows && x < p.cols) p.out[((int64_t)t.b * p.rows + y) * p.cols + x] = __ushort_as_bfloat16(0x7fff);
+  if (*s.abort_flag) ns_give_up<MODE>(p, w0, dw, pr);
+  cluster_sync_all();                            // nobody leaves while the pair's other CTA may still signal or read this one
+  if (warp == 1) { tc_fence_after(); tmem_dealloc_cg2(tmem_base, 2 * NS_T); }
+}
+
+// Few tiles: a cluster of S pairs per tile, each with a part of the k-blocks.  The partial sums cross the cluster as bulk copies
+// between shared memories, a warp's 32 rows at a time (stores of the drain's threads, one row each, took 9400 of 24000 cycles);
+// pair s finishes columns [s, s+1) * 256 / S and sums in pair order.
+// Shared memory: three stages (the copies leave from them), the partial sums that arrive, slots.
+constexpr int NS_SP_STAGES = 3, NS_OFF_PART = 2 * NS_SP_STAGES * A_BYTES;
+template <int MODE, bool TALL, int S>
+__global__ void __launch_bounds__(NS_THREADS, 1)
+ns_split_kernel(const __grid_constant__ NsArgs p) {
+  constexpr int G = 4 / S;                       // sub-tiles of 64 columns that a CTA finishes
+  constexpr int PART = BM * 256;                 // bytes of a partial sub-tile: [128 rows][64 columns] fp32
+  constexpr int OFF_SLOT = NS_OFF_PART + (S - 1) * G * PART;
+  static_assert((S - 1) * G * PART <= NS_OFF_PART, "what leaves fits into the stages");
+  static_assert(OFF_SLOT + G * 2 * C_SUB <= NS_OFF_BAR, "what arrives and the slots fit behind them");
+  unsigned char* smem = ns_smem();
+  const NsBars s(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pr = (int)(rank & 1u), sp = (int)(rank >> 1);
+  const uint32_t leader = rank & ~1u;
+  const uint16_t pair_mask = (uint16_t)(3u << leader);
+  const int64_t w = blockIdx.x / (2 * S);
+  pdl_launch_next();
+  if (threadIdx.x == 0) {
+    s.init();
+    mbar_expect_tx(s.pfull, (S - 1) * G * PART);
+    prefetch_tmap(&p.a.r128); prefetch_tmap(&p.a.r64); prefetch_tmap(&p.b.r128); prefetch_tmap(&p.b.r64);
+    prefetch_tmap(&p.s_hi); prefetch_tmap(&p.c_hi);
+  }
+  if (warp == 1) { tmem_alloc_cg2(s.tmem_slot, NS_T); tmem_relinquish_cg2(); }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = *s.tmem_slot;
+  pdl_wait();
+  const NsTile t = ns_decode<MODE>(w, p.m_tiles, p.n_tiles);
+  const int k0 = p.k_blocks * sp / S, k1 = p.k_blocks * (sp + 1) / S;
+  const int row = (warp & 3) * 32 + lane, h = (warp - 4) >> 2;
+  const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+  const int y = t.i * NS_T + pr * BM, x0 = t.j * NS_T + sp * G * 64;
+  auto slot_at = [&](int i) { return smem + OFF_SLOT + i * 2 * C_SUB; };
+  auto exists = [&](int i) { return x0 + i * 64 < p.cols && y < p.rows; };
+  // A partial sub-tile: 8 KB per warp pair (32 rows), in it 4 KB per half of the columns: a warp's [32 rows][8 pieces of 16 bytes],
+  // the pieces swizzled by the row
+  auto piece = [&](unsigned char* part, int k) { return part + (warp & 3) * 8192 + h * 4096 + lane * 128 + ((k ^ (lane & 7)) << 4); };
+
+  if (warp == 0) {
+    if (elect_one()) {
+      PipeState ps;
+      ns_produce<MODE, TALL, NS_SP_STAGES>(smem, p, s, t, k0, k1, pr, leader, ps);
+    }
+  } else if (warp == 1) {
+    if (pr == 0 && elect_one()) {
+      PipeState ps;
+      if (ns_multiply<MODE, TALL, NS_SP_STAGES>(smem, s, t, k0, k1, tmem_base, pair_mask, ps))
+        umma_commit_cg2_mc(&s.tfull[0], pair_mask);
+    }
+  } else if (warp == 2) {
+    if (elect_one()) {
+      for (int i = 0; i < G; ++i) {
+        if (!p.has_s || !exists(i)) { mbar_arrive(&s.sfull[i]); continue; }
+        mbar_expect_tx(&s.sfull[i], p.has_lo ? 2 * C_SUB : C_SUB);
+        tma_load_3d(slot_at(i), &p.s_hi, &s.sfull[i], x0 + i * 64, y, t.b);
+        if (p.has_lo) tma_load_3d(slot_at(i) + C_SUB, &p.s_lo, &s.sfull[i], x0 + i * 64, y, t.b);
+      }
+      for (int i = 0; i < G; ++i) {
+        if (!mbar_wait(&s.cfull[i], 0, s.abort_flag)) break;
+        if (!exists(i)) continue;
+        tma_store_3d(&p.c_hi, slot_at(i), x0 + i * 64, y, t.b);
+        if (p.out_lo) tma_store_3d(&p.c_lo, slot_at(i) + C_SUB, x0 + i * 64, y, t.b);
+        tma_store_commit();
+      }
+      tma_store_wait_all();
+    }
+  } else if (warp >= 4) {
+    bool ok = mbar_wait<true>(&s.tfull[0], 0, s.abort_flag);     // this pair's products are done: its stages are free
+    __syncwarp();
+    tc_fence_after();
+    const float mine = k1 > k0 ? 1.f : 0.f;                     // without a k-block of its own nothing was accumulated
+#pragma unroll 1
+    for (int d = 1; d < S && ok; ++d) {
+      const int to = (sp + d) % S;
+      const int o = sp < to ? sp : sp - 1;       // this pair's place among the others of `to`
+#pragma unroll 1
+      for (int i = 0; i < G; ++i) {
+        unsigned char* out = smem + ((d - 1) * G + i) * PART;
+        float r[32];
+        tmem_ld32(lane_addr + (to * G + i) * 64 + h * 32, reinterpret_cast<uint32_t*>(r));
+        tmem_ld_wait();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          float4 v = make_float4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+          if (mine == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+          *reinterpret_cast<float4*>(piece(out, k)) = v;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          const int at = (warp & 3) * 8192 + h * 4096;
+          const uint32_t cta = (uint32_t)(2 * to + pr);
+          asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                       ::"r"(map_to_cta(smem + NS_OFF_PART + (o * G + i) * PART + at, cta)), "r"(smem_u32(out + at)), "r"(4096),
+                       "r"(map_to_cta(s.pfull, cta)) : "memory");
         }
       }
     }
+    const NsScale c = ns_scale<MODE>(p, t.b, p.out_bf16 && *p.status != 0);
+    ok = ok && mbar_wait<true>(s.pfull, 0, s.abort_flag);
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < G && ok; ++i) {
+      float r[32], v[32];
+      tmem_ld32(lane_addr + (sp * G + i) * 64 + h * 32, reinterpret_cast<uint32_t*>(r));
+      tmem_ld_wait();
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v[k] = 0.f;
+#pragma unroll
+      for (int o = 0; o < S; ++o) {
+        if (o == sp) {
+          if (mine != 0.f)
+#pragma unroll
+            for (int k = 0; k < 32; ++k) v[k] += r[k];
+        } else {
+          unsigned char* part = smem + NS_OFF_PART + ((o < sp ? o : o - 1) * G + i) * PART;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 f = *reinterpret_cast<const float4*>(piece(part, k));
+            v[4 * k] += f.x; v[4 * k + 1] += f.y; v[4 * k + 2] += f.z; v[4 * k + 3] += f.w;
+          }
+        }
+      }
+      ok = mbar_wait(&s.sfull[i], 0, s.abort_flag);
+      __syncwarp();
+      if (!ok) break;
+      ns_finish(p, c, v, slot_at(i), row, h);
+      fence_proxy_async_smem();
+      mbar_arrive(&s.cfull[i]);
+    }
   }
-  cluster_sync_all();                            // nobody leaves while the pair's other CTA may still signal or read this one
-  if (warp == 1) { tc_fence_after(); tmem_dealloc_cg2(tmem_base, 2 * NS_T); }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*s.abort_flag) ns_give_up<MODE>(p, w, p.n_work, pr);
+  cluster_sync_all();                            // nobody leaves while copies to or from its shared memory may be under way
+  if (warp == 1) { tc_fence_after(); tmem_dealloc_cg2(tmem_base, NS_T); }
 }
 
 // ---- matrices with a side of at most 128: everything in one launch ------------------------------------------------------
@@ -676,14 +868,52 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p, int cluster) {
 }
 
 // ---- way in: sum of squares, then f16 (two halves for fp32), in the orientation of u ----------------------------------
+// A unit is up to NS_UNIT elements of a row (of the whole matrix where its rows follow each other); a block takes units blockIdx.x,
+// + gridDim.x, ...  16-byte accesses where rows and pointers allow them.
+constexpr int NS_UNIT = 8192;
+template <typename T, typename F>
+__device__ __forceinline__ void ns_units(const T* src, int64_t row_stride, int64_t rows, int64_t cols, bool vec, F&& f) {
+  constexpr int VE = 16 / sizeof(T);
+  const int64_t per_row = (cols + NS_UNIT - 1) / NS_UNIT;
+  for (int64_t i = blockIdx.x; i < rows * per_row; i += gridDim.x) {
+    const int64_t r = per_row == 1 ? i : i / per_row, c0 = per_row == 1 ? 0 : i % per_row * NS_UNIT;
+    const int64_t end = min(cols, c0 + NS_UNIT);
+    const T* at = src + r * row_stride;
+    if (vec) {
+#pragma unroll 4
+      for (int64_t c = c0 + threadIdx.x * VE; c < end; c += 256 * VE) {
+        const uint4 w = *reinterpret_cast<const uint4*>(at + c);
+        const uint32_t x4[4] = {w.x, w.y, w.z, w.w};
+        float v[VE];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (sizeof(T) == 4) v[k] = __uint_as_float(x4[k]);
+          else { v[2 * k] = bf16_lo(x4[k]); v[2 * k + 1] = bf16_hi(x4[k]); }
+        }
+        f(r, c, v, std::integral_constant<int, VE>());
+      }
+    } else {
+#pragma unroll 4
+      for (int64_t c = c0 + threadIdx.x; c < end; c += 256) {
+        float v[1] = {to_f32<T>(at[c])};
+        f(r, c, v, std::integral_constant<int, 1>());
+      }
+    }
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256)
-ns_sumsq_kernel(const T* __restrict__ u, int64_t batch_stride, int64_t row_stride, int rows, int cols, float* __restrict__ partial) {
+ns_sumsq_kernel(const T* __restrict__ u, int64_t batch_stride, int64_t row_stride, int64_t rows, int64_t cols, int vec,
+                float* __restrict__ partial) {
   __shared__ float red[8];
-  const T* src = u + (int64_t)blockIdx.y * batch_stride;
+  pdl_launch_next();
+  pdl_wait();
   float s = 0.f;
-  for (int r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int c = threadIdx.x; c < cols; c += 256) { const float v = to_f32<T>(src[(int64_t)r * row_stride + c]); s = fmaf(v, v, s); }
+  ns_units(u + (int64_t)blockIdx.y * batch_stride, row_stride, rows, cols, vec != 0, [&](int64_t, int64_t, const float* v, auto n) {
+#pragma unroll
+    for (int i = 0; i < n.value; ++i) s = fmaf(v[i], v[i], s);
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
@@ -698,44 +928,62 @@ ns_sumsq_kernel(const T* __restrict__ u, int64_t batch_stride, int64_t row_strid
 // x * q with q the power of two that brings the norm into (2048, 4096]; t = 4096 / ((norm + eps) q) is left in t_out
 template <typename T>
 __global__ void __launch_bounds__(256)
-ns_enter_kernel(const T* __restrict__ u, int64_t batch_stride, int64_t row_stride, int rows, int cols, float eps,
-                const float* __restrict__ partial, int n_parts, __half* __restrict__ hi, __half* __restrict__ lo, int ld,
+ns_enter_kernel(const T* __restrict__ u, int64_t batch_stride, int64_t row_stride, int64_t rows, int64_t cols, int vec, float eps,
+                const float* __restrict__ partial, int n_parts, __half* __restrict__ hi, __half* __restrict__ lo, int64_t ld,
                 float* __restrict__ t_out, int* __restrict__ status) {
   __shared__ float q_s;
+  pdl_launch_next();
+  pdl_wait();
   const int64_t b = blockIdx.y;
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < 32) {
     float s = 0.f;
-    for (int p = 0; p < n_parts; ++p) s += partial[b * NS_MAX_PARTS + p];
-    const float norm = sqrtf(s) + eps;
-    int e = 0;
-    float q = 1.f;
-    if (norm > 0.f && norm < 3e38f) {
-      frexpf(norm, &e);                          // norm = f * 2^e, f in [0.5, 1)
-      q = ldexpf(1.f, 12 - e < 120 ? 12 - e : 120);
-    }
-    q_s = q;
-    if (blockIdx.x == 0) {
-      t_out[b] = NS_ONE / (norm * q);
-      if (b == 0) *status = 0;
+    for (int p = threadIdx.x; p < n_parts; p += 32) s += partial[b * NS_MAX_PARTS + p];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x == 0) {
+      const float norm = sqrtf(s) + eps;
+      int e = 0;
+      float q = 1.f;
+      if (norm > 0.f && norm < 3e38f) {
+        frexpf(norm, &e);                        // norm = f * 2^e, f in [0.5, 1)
+        q = ldexpf(1.f, 12 - e < 120 ? 12 - e : 120);
+      }
+      q_s = q;
+      if (blockIdx.x == 0) {
+        t_out[b] = NS_ONE / (norm * q);
+        if (b == 0 && status != nullptr) *status = 0;
+      }
     }
   }
   __syncthreads();
   const float q = q_s;
-  const T* src = u + b * batch_stride;
-  for (int r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int c = threadIdx.x; c < cols; c += 256) {
-      const float v = q * to_f32<T>(src[(int64_t)r * row_stride + c]);
-      const __half h = __float2half_rn(v);
-      const int64_t at = (b * rows + r) * ld + c;
-      hi[at] = h;
-      if (lo != nullptr) lo[at] = __float2half_rn((v - __half2float(h)) * NS_LO);
-    }
+  hi += b * rows * ld;
+  if (lo != nullptr) lo += b * rows * ld;
+  ns_units(u + b * batch_stride, row_stride, rows, cols, vec != 0, [&](int64_t r, int64_t c, float* v, auto n) {
+    constexpr int N = decltype(n)::value;
+    __half h[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) { v[i] *= q; h[i] = __float2half_rn(v[i]); }
+    __half* at = hi + r * ld + c;
+    if constexpr (N == 8) *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(h);
+    else if constexpr (N == 4) *reinterpret_cast<uint2*>(at) = *reinterpret_cast<uint2*>(h);
+    else at[0] = h[0];
+    if (lo == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = __float2half_rn((v[i] - __half2float(h[i])) * NS_LO);
+    at = lo + r * ld + c;
+    if constexpr (N == 8) *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(h);
+    else if constexpr (N == 4) *reinterpret_cast<uint2*>(at) = *reinterpret_cast<uint2*>(h);
+    else at[0] = h[0];
+  });
 }
 
 // ---- way out where the result's rows cannot be stored as tiles --------------------------------------------------------
 __global__ void __launch_bounds__(256)
 ns_leave_kernel(const __half* __restrict__ x, int ld, int rows, int cols, const int* __restrict__ status,
                 __nv_bfloat16* __restrict__ out) {
+  pdl_launch_next();
+  pdl_wait();
   const int64_t b = blockIdx.y;
   const bool failed = *status != 0;              // a wait gave up: no number is left to stand
   for (int r = blockIdx.x; r < rows; r += gridDim.x)
@@ -746,35 +994,105 @@ ns_leave_kernel(const __half* __restrict__ x, int ld, int rows, int cols, const 
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
-template <int MODE, bool TALL> static int ns_launch(NsArgs& p, int64_t batch, int k_dim, cudaStream_t st) {
-  auto kern = ns_product_kernel<MODE, TALL>;
-  static DeviceOnce once;
-  const int rc = once.get([&](int*) {
+// a kernel that may start under the tail of the one before it
+template <typename Kern, typename... Args>
+static int ns_start(Kern kern, dim3 grid, int threads, int smem, int cluster, cudaStream_t st, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  BIBO_CUDA(cudaLaunchKernelEx(&cfg, kern, args...));
+  BIBO_CHECK_LAUNCH("orthogonalize");
+  return BIBO_OK;
+}
+template <typename Kern> static int ns_attributes(DeviceOnce& once, Kern kern) {
+  return once.get([&](int*) {
     BIBO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM));
     return (int)BIBO_OK;
   });
-  if (rc) return rc;
+}
+// how many clusters of S pairs are resident at once
+template <int MODE, bool TALL, int S> static int ns_split_resident(int* clusters) {
+  static DeviceOnce once;
+  return once.get([&](int* v) {
+    auto kern = ns_split_kernel<MODE, TALL, S>;
+    BIBO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * S);
+    cfg.blockDim = dim3(NS_THREADS);
+    cfg.dynamicSmemBytes = NS_SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2 * S;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    BIBO_CUDA(cudaOccupancyMaxActiveClusters(v, kern, &cfg));
+    return (int)BIBO_OK;
+  }, clusters);
+}
+template <int MODE, bool TALL, int S> static int ns_launch_split(const NsArgs& p, cudaStream_t st) {
+  return ns_start(ns_split_kernel<MODE, TALL, S>, dim3((unsigned)p.n_work * 2 * S), NS_THREADS, NS_SMEM, 2 * S, st, p);
+}
+template <int MODE, bool TALL> static int ns_launch(NsArgs& p, int64_t batch, int k_dim, cudaStream_t st) {
   p.m_tiles = (p.rows + NS_T - 1) / NS_T;
   p.n_tiles = (p.cols + NS_T - 1) / NS_T;
   p.k_blocks = (k_dim + BK - 1) / BK;
   p.n_work = batch * (MODE == NS_APPLY ? (int64_t)p.m_tiles * p.n_tiles : (int64_t)p.m_tiles * (p.m_tiles + 1) / 2);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(sm_count() / 2, p.n_work));
-  cfg.blockDim = dim3(NS_THREADS);
-  cfg.dynamicSmemBytes = NS_SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  BIBO_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
-  BIBO_CHECK_LAUNCH("ns_product_kernel");
-  return BIBO_OK;
+  // tiles so few that clusters of four (two) pairs for each are resident together are split over them
+  int four = 0, two = 0;
+  int rc = ns_split_resident<MODE, TALL, 4>(&four);
+  if (!rc) rc = ns_split_resident<MODE, TALL, 2>(&two);
+  if (rc) return rc;
+  if (p.n_work <= four) return ns_launch_split<MODE, TALL, 4>(p, st);
+  if (p.n_work <= two) return ns_launch_split<MODE, TALL, 2>(p, st);
+  static DeviceOnce once;
+  rc = ns_attributes(once, ns_product_kernel<MODE, TALL>);
+  return rc ? rc : ns_start(ns_product_kernel<MODE, TALL>, dim3(2 * (unsigned)std::min<int64_t>(sm_count() / 2, p.n_work)), NS_THREADS,
+                            NS_SMEM, 2, st, p);
 }
 template <int MODE> static int ns_product(NsArgs& p, int tall, int64_t batch, int k_dim, cudaStream_t st) {
   return tall ? ns_launch<MODE, true>(p, batch, k_dim, st) : ns_launch<MODE, false>(p, batch, k_dim, st);
+}
+
+// sums of squares and scaled x of nb matrices, in groups whose u (48 MB at most) is still in L2 for the second reading
+template <typename T>
+static int ns_enter(const T* u, int64_t nb, int64_t batch_stride, int rows, int cols, int64_t row_stride, float eps, float* partial,
+                    __half* hi, __half* lo, int ldx, float* t, int* status, cudaStream_t st) {
+  const int64_t bytes = (int64_t)rows * cols * sizeof(T);
+  const int64_t group = std::max<int64_t>(1, std::min<int64_t>(nb, (48 << 20) / bytes));
+  const bool whole_in = row_stride == cols || rows == 1, whole = whole_in && ldx == cols;   // rows follow each other: one long row
+  const bool vec = ((reinterpret_cast<uintptr_t>(u) | (uintptr_t)(batch_stride * sizeof(T))) & 15) == 0 && cols * sizeof(T) % 16 == 0 &&
+                   (whole_in || row_stride * sizeof(T) % 16 == 0);
+  auto blocks = [&](bool one, int64_t n) {
+    const int64_t units = one ? ((int64_t)rows * cols + NS_UNIT - 1) / NS_UNIT : (int64_t)rows * ((cols + NS_UNIT - 1) / NS_UNIT);
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>({units, NS_MAX_PARTS, (8 * (int64_t)sm_count() + n - 1) / n}));
+  };
+  for (int64_t g0 = 0; g0 < nb; g0 += group) {
+    const int64_t n = std::min(group, nb - g0);
+    const T* src = u + g0 * batch_stride;
+    const unsigned parts = blocks(whole_in, n);
+    int rc = ns_start(ns_sumsq_kernel<T>, dim3(parts, (unsigned)n), 256, 0, 1, st, src, batch_stride, row_stride,
+                      whole_in ? (int64_t)1 : (int64_t)rows, whole_in ? (int64_t)rows * cols : (int64_t)cols, (int)vec,
+                      partial + g0 * NS_MAX_PARTS);
+    if (rc) return rc;
+    rc = ns_start(ns_enter_kernel<T>, dim3(blocks(whole, n), (unsigned)n), 256, 0, 1, st, src, batch_stride, row_stride,
+                  whole ? (int64_t)1 : (int64_t)rows, whole ? (int64_t)rows * cols : (int64_t)cols, (int)vec, eps,
+                  (const float*)(partial + g0 * NS_MAX_PARTS), (int)parts, hi + g0 * rows * ldx,
+                  lo ? lo + g0 * rows * ldx : (__half*)nullptr, whole ? (int64_t)rows * ldx : (int64_t)ldx, t + g0,
+                  g0 == 0 ? status : (int*)nullptr);
+    if (rc) return rc;
+  }
+  return BIBO_OK;
 }
 
 // workspace of `batch` matrices: x twice and its lower half, four m x m matrices (f16, rows of 16-byte multiples), partial sums, t,
@@ -907,21 +1225,12 @@ extern "C" int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batc
     int* status = reinterpret_cast<int*>(ws + l.off_status);
     __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(out) + b0 * rows * cols;
     const unsigned char* src = static_cast<const unsigned char*>(u) + b0 * batch_stride * size;
-    const int parts = std::min(NS_MAX_PARTS, rows);
-    const dim3 sum_grid(parts, (unsigned)nb), row_grid(std::min(rows, 65535), (unsigned)nb);
-    if (dtype == BIBO_F32) {
-      ns_sumsq_kernel<float><<<sum_grid, 256, 0, st>>>(reinterpret_cast<const float*>(src), batch_stride, row_stride, rows, cols, partial);
-      BIBO_CHECK_LAUNCH("ns_sumsq_kernel");
-      ns_enter_kernel<float><<<row_grid, 256, 0, st>>>(reinterpret_cast<const float*>(src), batch_stride, row_stride, rows, cols, eps,
-                                                      partial, parts, x[0], x[2], l.ldx, t, status);
-    } else {
-      ns_sumsq_kernel<__nv_bfloat16><<<sum_grid, 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(src), batch_stride, row_stride,
-                                                              rows, cols, partial);
-      BIBO_CHECK_LAUNCH("ns_sumsq_kernel");
-      ns_enter_kernel<__nv_bfloat16><<<row_grid, 256, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(src), batch_stride, row_stride,
-                                                              rows, cols, eps, partial, parts, x[0], nullptr, l.ldx, t, status);
-    }
-    BIBO_CHECK_LAUNCH("ns_enter_kernel");
+    const int rc0 = dtype == BIBO_F32
+                        ? ns_enter(reinterpret_cast<const float*>(src), nb, batch_stride, rows, cols, row_stride, eps, partial, x[0], x[2],
+                                   l.ldx, t, status, st)
+                        : ns_enter(reinterpret_cast<const __nv_bfloat16*>(src), nb, batch_stride, rows, cols, row_stride, eps, partial,
+                                   x[0], nullptr, l.ldx, t, status, st);
+    if (rc0) return rc0;
     NsMaps mx[3], mm[4];                     // x, x', lower half;  m x m matrices
     CUtensorMap mout;
     int rc;
@@ -1006,8 +1315,9 @@ extern "C" int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batc
       ts = nullptr;
     }
     if (!direct) {
-      ns_leave_kernel<<<row_grid, 256, 0, st>>>(x[at], l.ldx, rows, cols, status, dst);
-      BIBO_CHECK_LAUNCH("ns_leave_kernel");
+      if ((rc = ns_start(ns_leave_kernel, dim3(std::min(rows, 65535), (unsigned)nb), 256, 0, 1, st, (const __half*)x[at], l.ldx, rows,
+                         cols, (const int*)status, dst)))
+        return rc;
     }
   }
   return BIBO_OK;

@@ -251,6 +251,11 @@ __device__ __forceinline__ void umma_commit_cg2_mc(uint64_t* bar, uint16_t cta_m
       : "memory");
 }
 
+// Programmatic dependent launch: a kernel launched with the attribute may start while the one before it in the stream still
+// runs; pdl_wait returns when that one is complete and its writes are visible (at once without the attribute).
+__device__ __forceinline__ void pdl_launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // named barrier among `n` threads (ids 1..15; 0 is __syncthreads)
 __device__ __forceinline__ void named_bar_sync(int id, int n) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory");

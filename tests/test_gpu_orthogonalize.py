@@ -74,11 +74,15 @@ def _check(u, steps=5, coefficients=NS, **kw):
     again = Fn.orthogonalize(u, steps, coefficients, **kw)
     torch.cuda.synchronize()
     assert got.dtype == torch.bfloat16 and got.shape == u.shape and got.is_contiguous() and torch.equal(got, again)
+    _near(got, u, steps, coefficients, **kw)
+    return got
+
+
+def _near(got, u, steps=5, coefficients=NS, **kw):
     want, bound = _steps64(u, steps, coefficients, **kw)
     diff = (got.double() - want).flatten(-2).norm(dim=-1)
     tol = 4 * bound + 2.0 ** -8 * want.flatten(-2).norm(dim=-1)
     assert bool((diff <= tol).all()), (diff / want.flatten(-2).norm(dim=-1), tol / want.flatten(-2).norm(dim=-1))
-    return got
 
 
 def _momentum(shape, dtype, seed, rank=8, floor=0.1, scale=1e-3):
@@ -166,8 +170,8 @@ def test_many_matrices():
     assert size(320, 640, 1024) == size(10000, 640, 1024) > 1 << 30       # a group of fewer than 320
     u = _momentum((320, 640, 1024), torch.bfloat16, 3)
     got = Fn.orthogonalize(u)
-    for i in (0, 150, 297, 298, 299, 300, 319):
-        assert torch.equal(got[i], Fn.orthogonalize(u[i]))
+    which = [0, 150, 297, 298, 299, 300, 319]
+    _near(got[which], u[which])                       # one matrix alone is summed in another order: not the same bits
 
 
 def test_two_graphs_and_streams_do_not_share_a_workspace():
