@@ -8,6 +8,8 @@
 //             dw[t,j] = <ys[slot_row[t,j]], dout[t]>, other rows of dys zero
 // A negative index is an empty slot: it has no row, its weight is not read and its dw is 0.  An index >= E is treated
 // the same way and raises the plan's status word.  Sums are fp32 in slot order: results do not depend on timing.
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace bibo {
@@ -364,41 +366,45 @@ dispatch_combine_kernel(const T* __restrict__ ys, const void* __restrict__ weigh
   const int c_lo = parts == 1 ? 0 : (int)(wi % parts) * part * 32, c_hi = min(chunks, c_lo + part * 32);
   SlotRows<V, K> rows;
   if (ONCE) rows.get(src, mine, my_w, 0, chunks);
-  for (int c0 = c_lo + lane; c0 - lane < c_hi; c0 += 32 * U) {
-    float acc[U][X::N];
+  // N accesses from column c on: all of them exist, or (N == 1) this lane's may not
+  auto block = [&](int c, auto n, bool in) {
+    constexpr int N = decltype(n)::value;
+    float acc[N][X::N];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < N; ++u)
 #pragma unroll
       for (int i = 0; i < X::N; ++i) acc[u][i] = 0.f;
     for (int j0 = 0; j0 < (ONCE ? 1 : top_k); j0 += K) {
       if (!ONCE) rows.get(src, mine, my_w, j0, chunks);
-      V v[U][K];
+      V v[N][K];
 #pragma unroll
       for (int j = 0; j < K; ++j)
-        if (rows.row[j] != nullptr)
+        if (rows.row[j] != nullptr && in)
 #pragma unroll
-          for (int u = 0; u < U; ++u)
-            if (c0 + u * 32 < c_hi) v[u][j] = __ldcs(rows.row[j] + c0 + u * 32);
+          for (int u = 0; u < N; ++u) v[u][j] = __ldcs(rows.row[j] + c + u * 32);
 #pragma unroll
       for (int j = 0; j < K; ++j)
-        if (rows.row[j] != nullptr)
+        if (rows.row[j] != nullptr && in)
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
+          for (int u = 0; u < N; ++u) {
             float f[X::N];
-            X::unpack(v[u][j], f);             // beyond c_hi: whatever the register holds, not stored
+            X::unpack(v[u][j], f);
 #pragma unroll
             for (int i = 0; i < X::N; ++i) acc[u][i] = fmaf(f[i], rows.w[j], acc[u][i]);
           }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c0 + u * 32 < c_hi) dst[c0 + u * 32] = X::pack(acc[u]);
-  }
+    for (int u = 0; u < N; ++u)
+      if (in) dst[c + u * 32] = X::pack(acc[u]);
+  };
+  int c = c_lo;
+  for (; c + 32 * U <= c_hi; c += 32 * U) block(c + lane, std::integral_constant<int, U>(), true);
+  for (; c < c_hi; c += 32) block(c + lane, std::integral_constant<int, 1>(), c + lane < c_hi);
 }
 
 // dys rows and dw of a token's slots, WPT warps per token (more for few tokens) that share its columns; blocks behind the tokens'
 // zero the rows of dys without a slot
-template <typename T, int VB, int K, int WPT>
+template <typename T, int VB, int K, int WPT, int U>
 __global__ void __launch_bounds__(DW * 32)
 dispatch_combine_bwd_kernel(const T* __restrict__ dout, int64_t dout_stride, const T* __restrict__ ys,
                             const void* __restrict__ weight, int w_bf16, const int32_t* __restrict__ slot_row,
@@ -428,28 +434,40 @@ dispatch_combine_bwd_kernel(const T* __restrict__ dout, int64_t dout_stride, con
       float dot[K];
 #pragma unroll
       for (int j = 0; j < K; ++j) dot[j] = 0.f;
-      for (int c = (warp % WPT) * 32 + lane; c < chunks; c += 32 * WPT) {
-        const V gv = g[c];
-        V v[K];
+      // N accesses, 32 * WPT columns apart, from column c on
+      auto block = [&](int c, auto n) {
+        constexpr int N = decltype(n)::value;
+        V gv[N], v[N][K];
+#pragma unroll
+        for (int u = 0; u < N; ++u) gv[u] = g[c + u * 32 * WPT];
 #pragma unroll
         for (int j = 0; j < K; ++j)
-          if (want && rows.row[j] != nullptr) v[j] = __ldcs(rows.row[j] + c);
-        float gf[X::N];
-        X::unpack(gv, gf);
+          if (want && rows.row[j] != nullptr)
+#pragma unroll
+            for (int u = 0; u < N; ++u) v[u][j] = __ldcs(rows.row[j] + c + u * 32 * WPT);
 #pragma unroll
         for (int j = 0; j < K; ++j)
           if (rows.row[j] != nullptr) {
-            float f[X::N];
-            if (want) {
-              X::unpack(v[j], f);
+            V* d = dst + (rows.row[j] - src);
 #pragma unroll
-              for (int i = 0; i < X::N; ++i) dot[j] = fmaf(gf[i], f[i], dot[j]);
+            for (int u = 0; u < N; ++u) {
+              float gf[X::N], f[X::N];
+              X::unpack(gv[u], gf);
+              if (want) {
+                X::unpack(v[u][j], f);
+#pragma unroll
+                for (int i = 0; i < X::N; ++i) dot[j] = fmaf(gf[i], f[i], dot[j]);
+              }
+#pragma unroll
+              for (int i = 0; i < X::N; ++i) f[i] = gf[i] * rows.w[j];
+              d[c + u * 32 * WPT] = X::pack(f);
             }
-#pragma unroll
-            for (int i = 0; i < X::N; ++i) f[i] = gf[i] * rows.w[j];
-            dst[rows.row[j] - src + c] = X::pack(f);
           }
-      }
+      };
+      int c = (warp % WPT) * 32 + lane;
+      for (; c + (U - 1) * 32 * WPT < chunks; c += U * 32 * WPT) block(c, std::integral_constant<int, U>());
+      if (U > 1)
+        for (; c < chunks; c += 32 * WPT) block(c, std::integral_constant<int, 1>());
       if (want) {
 #pragma unroll
         for (int j = 0; j < K; ++j) {
@@ -600,10 +618,11 @@ static void combine_v(const void* ys, const void* weight, int w_bf16, const int3
 #define BIBO_COMBINE(K, U, ONCE)                                                                                            \
   dispatch_combine_kernel<T, VB, K, U, ONCE><<<grid, DW * 32, 0, st>>>(static_cast<const T*>(ys), weight, w_bf16, slot_row, n_tokens, \
                                                                  top_k, chunks, parts, part, static_cast<T*>(out))
-  constexpr int M = VB == 16 ? 1 : 2;            // narrow accesses: more of them in flight
+  constexpr int M = VB == 16 ? 1 : 4;            // narrow accesses: more of them in flight
   if (top_k == 1) BIBO_COMBINE(1, 4 * M, true);
   else if (top_k == 2) BIBO_COMBINE(2, 4 * M, true);
-  else if (top_k <= 4) BIBO_COMBINE(4, 2 * M, true);
+  else if (top_k == 3) BIBO_COMBINE(3, 2 * M, true);
+  else if (top_k == 4) BIBO_COMBINE(4, 2 * M, true);
   else if (top_k <= 6) BIBO_COMBINE(6, 2 * M, true);
   else if (top_k <= 8) BIBO_COMBINE(8, 2 * M, true);
   else BIBO_COMBINE(8, 2 * M, false);
@@ -647,8 +666,9 @@ static void combine_bwd_v(const void* dout, int64_t dout_stride, const void* ys,
   const int wpt = n_tokens >= want ? 1 : 4 * n_tokens >= want ? 4 : DW;
   const int64_t token_blocks = (n_tokens * wpt + DW - 1) / DW;
   const unsigned grid = (unsigned)token_blocks + dispatch_grid((rows + DZ_ROWS - 1) / DZ_ROWS);
+  constexpr int M = VB == 16 ? 1 : 4;            // narrow accesses: more of them in flight
 #define BIBO_COMBINE_W(K, WPT)                                                                                               \
-  dispatch_combine_bwd_kernel<T, VB, K, WPT><<<grid, DW * 32, 0, st>>>(static_cast<const T*>(dout), dout_stride,             \
+  dispatch_combine_bwd_kernel<T, VB, K, WPT, M><<<grid, DW * 32, 0, st>>>(static_cast<const T*>(dout), dout_stride,             \
                                                                        static_cast<const T*>(ys), weight, w_bf16, slot_row,  \
                                                                        row_slot, n_tokens, top_k, rows, chunks, token_blocks, \
                                                                        static_cast<T*>(dys), dweight)
@@ -660,7 +680,8 @@ static void combine_bwd_v(const void* dout, int64_t dout_stride, const void* ys,
   } while (0)
   if (top_k == 1) BIBO_COMBINE(1);
   else if (top_k == 2) BIBO_COMBINE(2);
-  else if (top_k <= 4) BIBO_COMBINE(4);
+  else if (top_k == 3) BIBO_COMBINE(3);
+  else if (top_k == 4) BIBO_COMBINE(4);
   else if (top_k <= 6) BIBO_COMBINE(6);
   else BIBO_COMBINE(8);
 #undef BIBO_COMBINE_W

@@ -65,6 +65,7 @@ struct NsArgs {
   int m_tiles, n_tiles, k_blocks;
   int rows, cols;            // of the result
   int has_s, has_lo, out_lo; // source; source's or second source's map s_lo; result in two halves
+  int backwards;             // the tiles in reverse: what the launch before wrote last is still in L2 and is read first
   int out_bf16;              // the last product: c_hi is the caller's bf16 result
   float alpha, beta, beta_lo;   // C = alpha A B + beta S_hi + beta_lo S_lo
   const float* t_scale;      // first products: t of each matrix
@@ -73,7 +74,9 @@ struct NsArgs {
 };
 
 struct NsTile { int b, i, j; };
-template <int MODE> __device__ __forceinline__ NsTile ns_decode(int64_t w, int m_tiles, int n_tiles) {
+template <int MODE> __device__ __forceinline__ NsTile ns_decode(int64_t w, const NsArgs& p) {
+  const int m_tiles = p.m_tiles, n_tiles = p.n_tiles;
+  if (p.backwards) w = p.n_work - 1 - w;
   NsTile t;
   if (MODE == NS_APPLY) {
     const int64_t per = (int64_t)m_tiles * n_tiles;
@@ -255,7 +258,7 @@ template <int MODE> __device__ __forceinline__ void ns_give_up(const NsArgs& p, 
   if (threadIdx.x == 0) atomicExch(p.status, 112);
   if (!p.out_bf16) return;
   for (int64_t w = w0; w < p.n_work; w += dw) {
-    const NsTile t = ns_decode<MODE>(w, p.m_tiles, p.n_tiles);
+    const NsTile t = ns_decode<MODE>(w, p);
     for (int i = threadIdx.x; i < BM * NS_T; i += NS_THREADS) {
       const int y = t.i * NS_T + pr * BM + i / NS_T, x = t.j * NS_T + i % NS_T;
       if (y < p.rows && x < p.cols) p.out[((int64_t)t.b * p.rows + y) * p.cols + x] = __ushort_as_bfloat16(0x7fff);
@@ -297,7 +300,7 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
       PipeState ps;
       bool ok = true;
       for (int64_t w = w0; w < p.n_work && ok; w += dw)
-        ok = ns_produce<MODE, TALL>(smem, p, s, ns_decode<MODE>(w, p.m_tiles, p.n_tiles), 0, p.k_blocks, pr, 0, ps);
+        ok = ns_produce<MODE, TALL>(smem, p, s, ns_decode<MODE>(w, p), 0, p.k_blocks, pr, 0, ps);
     }
   } else if (warp == 1) {
     if (pr == 0 && elect_one()) {
@@ -307,7 +310,7 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
       for (int64_t w = w0; w < p.n_work; w += dw) {
         if (!mbar_wait<true>(&s.tempty[acc], acc_phase ^ 1, s.abort_flag)) break;
         tc_fence_after();
-        if (!ns_multiply<MODE, TALL>(smem, s, ns_decode<MODE>(w, p.m_tiles, p.n_tiles), 0, p.k_blocks, tmem_base + acc * NS_T, 3, ps)) break;
+        if (!ns_multiply<MODE, TALL>(smem, s, ns_decode<MODE>(w, p), 0, p.k_blocks, tmem_base + acc * NS_T, 3, ps)) break;
         umma_commit_cg2_mc(&s.tfull[acc], 3);
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
@@ -318,7 +321,7 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
       // sub-tile u of this CTA: tile w0 + (u / 4) * dw, columns (u % 4) * 64; a sub-tile outside the result is passed through
       const int64_t n_sub = w0 < p.n_work ? ((p.n_work - 1 - w0) / dw + 1) * 4 : 0;
       auto place = [&](int64_t u, NsTile& t, int& x, int& y) {
-        t = ns_decode<MODE>(w0 + (u >> 2) * dw, p.m_tiles, p.n_tiles);
+        t = ns_decode<MODE>(w0 + (u >> 2) * dw, p);
         x = t.j * NS_T + (int)(u & 3) * 64;
         y = t.i * NS_T + pr * BM;
         return x < p.cols && y < p.rows;
@@ -360,7 +363,7 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
     int64_t u = 0;
     bool ok = true;
     for (int64_t w = w0; w < p.n_work && ok; w += dw) {
-      const NsScale c = ns_scale<MODE>(p, ns_decode<MODE>(w, p.m_tiles, p.n_tiles).b, poison);
+      const NsScale c = ns_scale<MODE>(p, ns_decode<MODE>(w, p).b, poison);
       ok = mbar_wait<true>(&s.tfull[acc], acc_phase, s.abort_flag);
       if (!ok) break;
       __syncwarp();
@@ -429,7 +432,7 @@ ns_split_kernel(const __grid_constant__ NsArgs p) {
   tc_fence_after();
   const uint32_t tmem_base = *s.tmem_slot;
   pdl_wait();
-  const NsTile t = ns_decode<MODE>(w, p.m_tiles, p.n_tiles);
+  const NsTile t = ns_decode<MODE>(w, p);
   const int k0 = p.k_blocks * sp / S, k1 = p.k_blocks * (sp + 1) / S;
   const int row = (warp & 3) * 32 + lane, h = (warp - 4) >> 2;
   const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
@@ -1243,8 +1246,10 @@ extern "C" int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batc
 
     NsArgs base = {};
     base.status = status;
+    base.backwards = 0;
     auto gram = [&](int from, int to, const float* ts) {
       NsArgs p = base;
+      base.backwards ^= 1;
       p.a = p.b = mx[from];
       p.s_hi = p.s_lo = p.c_hi = p.c_lo = mm[to].r128;
       p.rows = p.cols = l.m;
@@ -1255,6 +1260,7 @@ extern "C" int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batc
     // mm[to] = alpha mm[a] mm[b] + beta mm[s] + beta2 mm[s2]
     auto sym = [&](int a, int b, float alpha, int s, float beta, int s2, float beta2, int to) {
       NsArgs p = base;
+      base.backwards ^= 1;
       p.a = mm[a];
       p.b = mm[b];
       p.s_hi = mm[s].r128;
@@ -1271,6 +1277,7 @@ extern "C" int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batc
     // x[1 - from] = mm[f] x + a x
     auto apply = [&](int f, int from, float a, bool lo_in, bool lo_out, bool last, const float* ts) {
       NsArgs p = base;
+      base.backwards ^= 1;
       p.a = tall ? mx[from] : mm[f];
       p.b = tall ? mm[f] : mx[from];
       p.s_hi = mx[from].r128;
