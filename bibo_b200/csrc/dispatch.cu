@@ -10,7 +10,7 @@
 // the same way and raises the plan's status word.  Sums are fp32 in slot order: results do not depend on timing.
 #include <type_traits>
 
-#include "common.cuh"
+#include "tc_common.cuh"
 
 namespace bibo {
 
@@ -169,6 +169,7 @@ dispatch_count_kernel(const I* __restrict__ idx, int64_t slots, int64_t per_bloc
   int32_t* hist = d.hists + (size_t)warp * d.pitch;
   if (threadIdx.x == 0) bad_s = 0;
   __syncthreads();
+  tc::pdl_launch_next();                     // dispatch_rows_kernel may be set up under this one
   const int64_t b0 = min(slots, blockIdx.x * per_block), b1 = min(slots, b0 + per_block);
   const int64_t per = ((b1 - b0 + warps - 1) / warps + 31) / 32 * 32, s0 = min(b1, b0 + warp * per), s1 = min(b1, s0 + per);
   dp_rank(idx, s0, s1, E, bits, hist, slot_row, &bad_s);
@@ -192,6 +193,7 @@ dispatch_rows_kernel(const I* __restrict__ idx, int64_t slots, int64_t per_block
   const int n = gridDim.x, b = blockIdx.x;
   for (int e = threadIdx.x; e < E; e += blockDim.x) d.count[e] = d.lower[e] = 0;
   __syncthreads();
+  tc::pdl_wait();
   // a thread adds up one expert over every `groups`-th block, then once into shared memory (whole numbers: any order)
   int ep = 32;
   while (ep < E) ep *= 2;
@@ -270,7 +272,7 @@ template <int VB> struct RowElems<__nv_bfloat16, VB> {
 };
 
 constexpr int DW = 8;          // warps per block
-constexpr int DZ_ROWS = 16;    // rows a warp looks at for zeroing
+constexpr int DZ_ROWS = 4;     // rows a warp looks at for zeroing (with 16 a tail of empty rows was left to a few hundred warps)
 
 // zeroes the rows of [r0, r0 + DZ_ROWS) that have no slot
 template <int VB>
@@ -543,7 +545,17 @@ static int plan_launch(const void* idx_, int64_t slots, int E, int align, int32_
   int32_t* scratch = plan + dp_off_scratch(slots, E, cap);
   dispatch_count_kernel<I><<<blocks, 1024, dp_smem(E, 1024), st>>>(idx, slots, per, E, bits, plan + dp_off_slot_row(E), scratch);
   BIBO_CHECK_LAUNCH("dispatch_count_kernel");
-  dispatch_rows_kernel<I><<<blocks, 1024, dp_smem(E, 0), st>>>(idx, slots, per, E, align, cap, scratch, plan);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(1024);
+  cfg.dynamicSmemBytes = dp_smem(E, 0);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  BIBO_CUDA(cudaLaunchKernelEx(&cfg, dispatch_rows_kernel<I>, idx, slots, per, E, align, cap, (const int32_t*)scratch, plan));
   BIBO_CHECK_LAUNCH("dispatch_rows_kernel");
   return BIBO_OK;
 }

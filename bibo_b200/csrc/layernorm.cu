@@ -196,6 +196,7 @@ layernorm_bwd_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restr
   constexpr int WARPS = NT / 32;
   __shared__ float red[2][WARPS * 2 * R];
   const int tid = threadIdx.x;
+  tc::pdl_launch_next();                   // layernorm_dparam_kernel may take its place beside this one and wait
   const int vecs = hidden / VE;
   const float inv = 1.f / (float)hidden;
   float dw[CH][VE], db[CH][VE];
@@ -203,6 +204,17 @@ layernorm_bwd_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restr
   for (int q = 0; q < CH; ++q)
 #pragma unroll
     for (int i = 0; i < VE; ++i) dw[q][i] = db[q][i] = 0.f;
+  // the parameters of a thread's columns stay in registers where they are few
+  constexpr bool KEEP = CH * VE <= 8;
+  float wk[KEEP ? CH : 1][VE];
+  auto param = [&](int q, float* w) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) w[i] = 1.f;
+    if (weight != nullptr && q * NT + tid < vecs) ln_param<W, VE>(weight, q * NT + tid, w);
+  };
+  if (KEEP)
+#pragma unroll
+    for (int q = 0; q < CH; ++q) param(q, wk[KEEP ? q : 0]);
   int buf = 0;
   for (int64_t row0 = (int64_t)blockIdx.x * R; row0 < n_rows; row0 += (int64_t)gridDim.x * R, buf ^= 1) {
     V xv[R][CH], gv[R][CH];
@@ -229,9 +241,10 @@ layernorm_bwd_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restr
         float f[VE], g[VE], w[VE];
         X::unpack(xv[r][q], f);
         X::unpack(gv[r][q], g);
+        if (KEEP)
 #pragma unroll
-        for (int i = 0; i < VE; ++i) w[i] = 1.f;
-        if (weight != nullptr && q * NT + tid < vecs) ln_param<W, VE>(weight, q * NT + tid, w);
+          for (int i = 0; i < VE; ++i) w[i] = wk[KEEP ? q : 0][i];
+        else param(q, w);
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
           const float z = (f[i] - mean[r]) * rstd[r], gw = g[i] * w[i];
@@ -257,9 +270,10 @@ layernorm_bwd_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restr
         float f[VE], g[VE], w[VE];
         X::unpack(xv[r][q], f);
         X::unpack(gv[r][q], g);
+        if (KEEP)
 #pragma unroll
-        for (int i = 0; i < VE; ++i) w[i] = 1.f;
-        if (weight != nullptr) ln_param<W, VE>(weight, c, w);
+          for (int i = 0; i < VE; ++i) w[i] = wk[KEEP ? q : 0][i];
+        else param(q, w);
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
           const float z = (f[i] - mean[r]) * rstd[r];
@@ -438,6 +452,7 @@ layernorm_bwd_ring_kernel(const T* __restrict__ x, int64_t x_stride, const T* __
   volatile int* abort_flag = &abort_s;
   const int tid = threadIdx.x, vecs = hidden / VE, row_bytes = hidden * (int)sizeof(T);
   const float inv = 1.f / (float)hidden;
+  tc::pdl_launch_next();                   // layernorm_dparam_kernel may take its place beside this one and wait
   const int64_t step = (int64_t)gridDim.x * R, first = (int64_t)blockIdx.x * R;
   auto load = [&](int64_t row0, int st) {                        // thread 0
     const int rows = n_rows - row0 < R ? (int)(n_rows - row0) : R;
@@ -669,6 +684,7 @@ layernorm_dparam_kernel(const float* __restrict__ partial, int n_parts, int hidd
   const int which = blockIdx.y;                 // 0: dweight, 1: dbias
   W* dst = which == 0 ? dweight : dbias;
   if (dst == nullptr) return;                   // the whole block
+  tc::pdl_wait();
   float s = 0.f;
   if (c < hidden) {
     const float* p = partial + (int64_t)which * hidden + c;
@@ -880,8 +896,17 @@ static int layernorm_bwd_t(const void* x, int64_t x_stride, const void* dy, int6
     BIBO_CHECK_LAUNCH("layernorm_bwd_cols_kernel");
   }
   if (!params) return BIBO_OK;
-  layernorm_dparam_kernel<W><<<dim3((hidden + 31) / 32, 2), 1024, 0, st>>>(partial, used, hidden, static_cast<W*>(dweight),
-                                                                        static_cast<W*>(dbias));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((hidden + 31) / 32, 2);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  BIBO_CUDA(cudaLaunchKernelEx(&cfg, layernorm_dparam_kernel<W>, (const float*)partial, used, hidden, static_cast<W*>(dweight),
+                               static_cast<W*>(dbias)));
   BIBO_CHECK_LAUNCH("layernorm_dparam_kernel");
   return BIBO_OK;
 }

@@ -586,9 +586,10 @@ struct NsSmallArgs {
   float coefficients[64 * 3];
 };
 
-template <typename T>
+template <typename T, int CLUSTER>
 __global__ void __launch_bounds__(NS_SM_THREADS, 1)
-ns_small_kernel(const __grid_constant__ NsSmallArgs p, int cluster) {
+ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
+  constexpr int cluster = CLUSTER;
   extern __shared__ unsigned char smem_dyn[];
   // the same offset in every CTA of the cluster: the dynamic shared memory starts at one address in all of them
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
@@ -708,8 +709,12 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p, int cluster) {
   if (cluster > 1) {
     if (threadIdx.x == 0) red[8] = ss;
     cluster_sync_all();
+    float part[cluster];
+#pragma unroll
+    for (int c = 0; c < cluster; ++c) part[c] = ld_remote_f1(red + 8, c);
     ss = 0.f;
-    for (int c = 0; c < cluster; ++c) ss += ld_remote_f1(red + 8, c);
+#pragma unroll
+    for (int c = 0; c < cluster; ++c) ss += part[c];
   }
   const float inv = 1.f / (sqrtf(ss) + p.eps);
   const float* co = p.coefficients;
@@ -761,13 +766,15 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p, int cluster) {
         const int r = (int)cta + i / quads * cluster, k = i % quads;
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
         const float4* at = reinterpret_cast<const float4*>(exch) + r * 32 + (k ^ (r & 7));
-        for (int c = 0; c < cluster; ++c) {
-          const float4 v = ld_remote_f4(at, c);
-          s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-        }
+        float4 v[cluster];
+#pragma unroll
+        for (int c = 0; c < cluster; ++c) v[c] = ld_remote_f4(at, c);
+#pragma unroll
+        for (int c = 0; c < cluster; ++c) { s.x += v[c].x; s.y += v[c].y; s.z += v[c].z; s.w += v[c].w; }
         const float z = 1.f / NS_ONE;
         const uint2 o = make_uint2(pack_f16(s.x * z, s.y * z), pack_f16(s.z * z, s.w * z));
         unsigned char* dst = mat + (k >> 4) * C_SUB + swz(r, (k & 15) >> 1) + (k & 1) * 8;
+#pragma unroll
         for (int c = 0; c < cluster; ++c) st_remote_u2(dst, c, o);
       }
       fence_proxy_async_all();
@@ -1135,10 +1142,11 @@ static int ns_small_cluster(int64_t batch, int rows, int cols) {
   while (c < NS_SM_MAX_CLUSTER && n >= 256 * c && batch * 2 * c <= sm_count()) c *= 2;
   return c;
 }
-template <typename T>
+template <typename T, int CLUSTER>
 static int ns_small(const void* u, int64_t batch, int64_t batch_stride, int rows, int cols, int64_t row_stride, int steps, bool joint,
-                    const float* co, float eps, int cluster, void* out, cudaStream_t st) {
-  auto kern = ns_small_kernel<T>;
+                    const float* co, float eps, void* out, cudaStream_t st) {
+  constexpr int cluster = CLUSTER;
+  auto kern = ns_small_kernel<T, CLUSTER>;
   static DeviceOnce once;
   const int rc = once.get([&](int*) {
     BIBO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SM_BYTES));
@@ -1173,7 +1181,7 @@ static int ns_small(const void* u, int64_t batch, int64_t batch_stride, int rows
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    BIBO_CUDA(cudaLaunchKernelEx(&cfg, kern, p, cluster));
+    BIBO_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
     BIBO_CHECK_LAUNCH("ns_small_kernel");
   }
   return BIBO_OK;
@@ -1214,10 +1222,13 @@ extern "C" int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batc
   const float* co = coefficients_host;
   // the first two steps as one, where their joint matrices stay in range (|T| <= a1^2, |R| <= a1 a2) and a step follows
   const bool joint = steps >= 3 && co[0] * co[0] <= 14.f && co[0] * co[3] <= 14.f && co[0] > 0.f && co[3] > 0.f;
-  if (cluster)
-    return dtype == BIBO_F32
-               ? ns_small<float>(u, batch, batch_stride, rows, cols, row_stride, steps, joint, co, eps, cluster, out, st)
-               : ns_small<__nv_bfloat16>(u, batch, batch_stride, rows, cols, row_stride, steps, joint, co, eps, cluster, out, st);
+#define BIBO_NS_SMALL(C)                                                                                                        \
+  if (cluster == C)                                                                                                             \
+    return dtype == BIBO_F32                                                                                                    \
+               ? ns_small<float, C>(u, batch, batch_stride, rows, cols, row_stride, steps, joint, co, eps, out, st)             \
+               : ns_small<__nv_bfloat16, C>(u, batch, batch_stride, rows, cols, row_stride, steps, joint, co, eps, out, st);
+  BIBO_NS_SMALL(1) BIBO_NS_SMALL(2) BIBO_NS_SMALL(4) BIBO_NS_SMALL(8)
+#undef BIBO_NS_SMALL
   for (int64_t b0 = 0; b0 < batch; b0 += chunk) {
     const int64_t nb = std::min(chunk, batch - b0);
     const NsLayout l(nb, rows, cols);
