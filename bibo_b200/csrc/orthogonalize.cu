@@ -61,7 +61,7 @@ struct NsMaps {            // a matrix of a batch with boxes of 128 rows (K-majo
 struct NsArgs {
   NsMaps a, b;
   CUtensorMap s_hi, s_lo, c_hi, c_lo;
-  int64_t n_work;
+  int64_t n_work, batch;
   int m_tiles, n_tiles, k_blocks;
   int rows, cols;            // of the result
   int has_s, has_lo, out_lo; // source; source's or second source's map s_lo; result in two halves
@@ -397,9 +397,10 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
   if (warp == 1) { tc_fence_after(); tmem_dealloc_cg2(tmem_base, 2 * NS_T); }
 }
 
-// Few tiles: a cluster of S pairs per tile, each with a part of the k-blocks.  The partial sums cross the cluster as bulk copies
+// Few tiles and a long k: a cluster of S pairs per tile, each with a part of the k-blocks.  The partial sums cross the cluster as bulk copies
 // between shared memories, a warp's 32 rows at a time (stores of the drain's threads, one row each, took 9400 of 24000 cycles);
-// pair s finishes columns [s, s+1) * 256 / S and sums in pair order.
+// pair s finishes columns [s, s+1) * 256 / S and sums in pair order.  4096 x 1024: the Gram product (k = 4096) 29 us on ten pairs
+// alone, 17 us split.
 // Shared memory: three stages (the copies leave from them), the partial sums that arrive, slots.
 constexpr int NS_SP_STAGES = 3, NS_OFF_PART = 2 * NS_SP_STAGES * A_BYTES;
 template <int MODE, bool TALL, int S>
@@ -542,6 +543,157 @@ ns_split_kernel(const __grid_constant__ NsArgs p) {
   if (*s.abort_flag) ns_give_up<MODE>(p, w, p.n_work, pr);
   cluster_sync_all();                            // nobody leaves while copies to or from its shared memory may be under way
   if (warp == 1) { tc_fence_after(); tmem_dealloc_cg2(tmem_base, NS_T); }
+}
+
+// Few tiles: one CTA per 128 x 128 tile.  The tiles of a 256 x 256 block on the diagonal are all computed, so that what the pairs'
+// kernel reads is there.
+constexpr int NS_ST_BN = 128;
+template <int MODE> __device__ __forceinline__ NsTile ns_decode_single(int64_t w, const NsArgs& p) {
+  NsTile t;
+  if (MODE == NS_APPLY) {
+    const int64_t per = (int64_t)p.m_tiles * p.n_tiles;
+    t.b = (int)(w / per);
+    const int r = (int)(w % per);
+    t.i = r % p.m_tiles;
+    t.j = r / p.m_tiles;
+  } else {
+    // rows 2 h and 2 h + 1 have 2 h + 2 tiles each (one less where the last row is alone): h (h + 1) * 2 tiles lie before them
+    const int per = (int)(p.n_work / p.batch);
+    t.b = (int)(w / per);
+    const int r = (int)(w % per);
+    int h = (int)((sqrtf(2.f * r + 1.f) - 1.f) * 0.5f);
+    while (2 * (h + 1) * (h + 2) <= r) ++h;
+    while (2 * h * (h + 1) > r) --h;
+    const int q = r - 2 * h * (h + 1), width = min(2 * h + 2, p.m_tiles);
+    t.i = 2 * h + q / width;
+    t.j = q % width;
+  }
+  return t;
+}
+template <int OP>
+__device__ __forceinline__ bool ns_load_single(unsigned char* dst, const NsMaps& m, uint64_t* bar, int tile, int kb, int b) {
+  const int r0 = tile * BM;
+  const bool mn = OP == OP_MN || (OP == OP_SYM && kb / (BM / BK) > tile);
+  if (mn) {
+    tma_load_3d(dst, &m.r64, bar, r0, kb * BK, b);
+    tma_load_3d(dst + MN_BOX, &m.r64, bar, r0 + 64, kb * BK, b);
+  } else {
+    tma_load_3d(dst, &m.r128, bar, kb * BK, r0, b);
+  }
+  return mn;
+}
+template <int MODE, bool TALL>
+__global__ void __launch_bounds__(NS_THREADS, 1)
+ns_single_kernel(const __grid_constant__ NsArgs p) {
+  using Ops = NsOps<MODE, TALL>;
+  unsigned char* smem = ns_smem();
+  const NsBars s(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_next();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS_STAGES; ++i) { mbar_init(&s.full[i], 1); mbar_init(&s.empty[i], 1); }
+    mbar_init(&s.tfull[0], 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&s.sfull[i], 1); mbar_init(&s.cfull[i], NS_DRAIN / 2); }
+    *s.abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&p.a.r128); prefetch_tmap(&p.a.r64); prefetch_tmap(&p.b.r128); prefetch_tmap(&p.b.r64);
+    prefetch_tmap(&p.s_hi); prefetch_tmap(&p.c_hi);
+  }
+  if (warp == 1) { tmem_alloc(s.tmem_slot, NS_ST_BN); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *s.tmem_slot;
+  const int64_t w = blockIdx.x;
+  const NsTile t = ns_decode_single<MODE>(w, p);
+  const bool same = Ops::same(t);
+  const int y = t.i * BM, x0 = t.j * NS_ST_BN;
+  auto slot_at = [&](int i) { return smem + NS_OFF_SLOT + i * 2 * C_SUB; };
+  pdl_wait();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      PipeState ps;
+      for (int kb = 0; kb < p.k_blocks; ++kb) {
+        if (!mbar_wait(&s.empty[ps.stage], ps.phase ^ 1, s.abort_flag)) break;
+        mbar_expect_tx(&s.full[ps.stage], same ? A_BYTES : 2 * A_BYTES);
+        ns_load_single<Ops::A>(smem + NS_OFF_A + ps.stage * A_BYTES, p.a, &s.full[ps.stage], t.i, kb, t.b);
+        if (!same) ns_load_single<Ops::B>(smem + NS_OFF_B + ps.stage * A_BYTES, p.b, &s.full[ps.stage], t.j, kb, t.b);
+        ps.next<NS_STAGES>();
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      PipeState ps;
+      bool ok = true;
+      for (int kb = 0; kb < p.k_blocks; ++kb) {
+        ok = mbar_wait(&s.full[ps.stage], ps.phase, s.abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t sa = smem_u32(smem + NS_OFF_A + ps.stage * A_BYTES);
+        const uint32_t sb = same ? sa : smem_u32(smem + NS_OFF_B + ps.stage * A_BYTES);
+        const bool amn = Ops::A == OP_MN || (Ops::A == OP_SYM && kb / (BM / BK) > t.i);
+        const bool bmn = Ops::B == OP_MN || (Ops::B == OP_SYM && kb / (BM / BK) > t.j);
+        const uint64_t da = amn ? make_sdesc_mn128(sa) : make_sdesc_k128(sa);
+        const uint64_t db = bmn ? make_sdesc_mn128(sb) : make_sdesc_k128(sb);
+        const int a_step = amn ? (2048 >> 4) : (32 >> 4), b_step = bmn ? (2048 >> 4) : (32 >> 4);
+        const uint32_t idesc = make_idesc_f16(BM, NS_ST_BN) | (amn ? 1u << 15 : 0u) | (bmn ? 1u << 16 : 0u);
+#pragma unroll
+        for (int k = 0; k < BK / UK; ++k) umma_bf16(tmem_base, da + k * a_step, db + k * b_step, idesc, (kb | k) != 0);
+        umma_commit(&s.empty[ps.stage]);
+        ps.next<NS_STAGES>();
+      }
+      if (ok) umma_commit(&s.tfull[0]);
+    }
+  } else if (warp == 2) {
+    if (elect_one()) {
+      for (int i = 0; i < 2; ++i) {
+        if (!p.has_s || x0 + i * 64 >= p.cols) { mbar_arrive(&s.sfull[i]); continue; }
+        mbar_expect_tx(&s.sfull[i], p.has_lo ? 2 * C_SUB : C_SUB);
+        tma_load_3d(slot_at(i), &p.s_hi, &s.sfull[i], x0 + i * 64, y, t.b);
+        if (p.has_lo) tma_load_3d(slot_at(i) + C_SUB, &p.s_lo, &s.sfull[i], x0 + i * 64, y, t.b);
+      }
+      for (int i = 0; i < 2; ++i) {
+        if (!mbar_wait(&s.cfull[i], 0, s.abort_flag)) break;
+        if (x0 + i * 64 >= p.cols) continue;
+        tma_store_3d(&p.c_hi, slot_at(i), x0 + i * 64, y, t.b);
+        if (p.out_lo) tma_store_3d(&p.c_lo, slot_at(i) + C_SUB, x0 + i * 64, y, t.b);
+        tma_store_commit();
+      }
+      tma_store_wait_all();
+    }
+  } else if (warp >= 4) {
+    const int row = (warp & 3) * 32 + lane, i = (warp - 4) >> 2;       // four warps per sub-tile of 64 columns
+    const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + i * 64;
+    const NsScale c = ns_scale<MODE>(p, t.b, p.out_bf16 && *p.status != 0);
+    bool ok = mbar_wait(&s.tfull[0], 0, s.abort_flag) && mbar_wait(&s.sfull[i], 0, s.abort_flag);
+    __syncwarp();
+    tc_fence_after();
+    if (ok) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float r[32];
+        tmem_ld32(lane_addr + h * 32, reinterpret_cast<uint32_t*>(r));
+        tmem_ld_wait();
+        ns_finish(p, c, r, slot_at(i), row, h);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&s.cfull[i]);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (*s.abort_flag) {
+    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+    if (threadIdx.x == 0) atomicExch(p.status, 112);
+    if (p.out_bf16)
+      for (int i = threadIdx.x; i < BM * NS_ST_BN; i += NS_THREADS) {
+        const int r = y + i / NS_ST_BN, x = x0 + i % NS_ST_BN;
+        if (r < p.rows && x < p.cols) p.out[((int64_t)t.b * p.rows + r) * p.cols + x] = __ushort_as_bfloat16(0x7fff);
+      }
+  }
+  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, NS_ST_BN); }
 }
 
 // ---- matrices with a side of at most 128: everything in one launch ------------------------------------------------------
@@ -691,12 +843,17 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
 
   // ---- x_0: raw values into tensor memory, their squares over the cluster, then scaled
   float ss = 0.f;
-  for (int g = half; g < groups; g += 2) {
-    float v[32];
-    load(g * 32, v);
+  for (int g = half; g < groups; g += 4) {       // two pieces of a thread's row in flight
+    float v[2][32];
+    load(g * 32, v[0]);
+    if (g + 2 < groups) load((g + 2) * 32, v[1]);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) ss = fmaf(v[i], v[i], ss);
-    tmem_st32(tx + lane_off + g * 32, reinterpret_cast<const uint32_t*>(v));
+    for (int k = 0; k < 2; ++k) {
+      if (g + 2 * k >= groups) break;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) ss = fmaf(v[k][i], v[k][i], ss);
+      tmem_st32(tx + lane_off + (g + 2 * k) * 32, reinterpret_cast<const uint32_t*>(v[k]));
+    }
   }
   tmem_st_wait();
 #pragma unroll
@@ -1058,6 +1215,26 @@ template <int MODE, bool TALL> static int ns_launch(NsArgs& p, int64_t batch, in
   p.n_tiles = (p.cols + NS_T - 1) / NS_T;
   p.k_blocks = (k_dim + BK - 1) / BK;
   p.n_work = batch * (MODE == NS_APPLY ? (int64_t)p.m_tiles * p.n_tiles : (int64_t)p.m_tiles * (p.m_tiles + 1) / 2);
+  p.batch = batch;
+  // 128 x 128 tiles that fit the machine at once, unless k is so long that splitting it over pairs gains more than the exchange
+  // costs.  All steps of 1024 x 1024: 151 us this way, 186 split, 218 with a pair per tile; of 512 x 8192: 249 us against 198.
+  if (p.k_blocks <= 40) {
+    const int mt = (p.rows + BM - 1) / BM, nt = (p.cols + NS_ST_BN - 1) / NS_ST_BN;
+    int64_t tiles = (int64_t)mt * nt;
+    if (MODE != NS_APPLY) {
+      tiles = 0;
+      for (int i = 0; i < mt; ++i) tiles += std::min(i / 2 * 2 + 2, mt);
+    }
+    if (batch * tiles <= sm_count()) {
+      NsArgs q = p;
+      q.m_tiles = mt;
+      q.n_tiles = nt;
+      q.n_work = batch * tiles;
+      static DeviceOnce once1;
+      const int rc1 = ns_attributes(once1, ns_single_kernel<MODE, TALL>);
+      return rc1 ? rc1 : ns_start(ns_single_kernel<MODE, TALL>, dim3((unsigned)q.n_work), NS_THREADS, NS_SMEM, 1, st, q);
+    }
+  }
   // tiles so few that clusters of four (two) pairs for each are resident together are split over them
   int four = 0, two = 0;
   int rc = ns_split_resident<MODE, TALL, 4>(&four);
