@@ -701,7 +701,9 @@ ns_single_kernel(const __grid_constant__ NsArgs p) {
 // tensor memory in fp32, times 2^24 and the next step's a, so that "a x + F x" is an accumulation onto it; its upper half in
 // f16 is the operand of both products, in one shared-memory layout that is K-major for x x^T and MN-major for F x.  The Gram
 // matrices of the slices are summed through distributed shared memory (each CTA reduces every C-th row and hands the rounded
-// result to all); the m x m products are done by every CTA for itself.  The launches, not the flops, are what a small matrix
+// result to all); the m x m products are done by every CTA for itself, for m <= 64 on matrices in two halves (22 bits: with n
+// much larger than m the singular values are alike and close to where the polynomial is steep, and the roundings of the m x m
+// matrices were most of the error, 0.0026 against 0.0017 at 19 x 1794).  The launches, not the flops, are what a small matrix
 // costs: 64 x 2048 fp32 took 18 launches and 211 us.
 constexpr int NS_SM_THREADS = 256, NS_SM_COLS = 384, NS_SM_MAX_CLUSTER = 8;
 constexpr int NS_MAT = 2 * C_SUB;                               // a 128 x 128 f16 matrix: two sub-tiles of 64 columns
@@ -766,6 +768,9 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
   const int m = p.m, mp = (m + 31) / 32 * 32, c0 = (int)cta * p.slice;
   const int cols = min(p.slice, max(0, p.n - c0));               // of this slice that exist
   const int groups = (cols + 63) / 64 * 2;                       // pieces of 32 columns, zero-filled up to 64
+  // Rows m .. mp are zeros throughout; what the tiles hold in rows beyond mp takes part in nothing (a product's row depends on
+  // that row of its first operand only, and the second's rows end at mp), so the warps of those rows leave them alone.
+  const bool mine = (warp & 3) * 32 < mp;
   uint32_t phase = 0;
 
   const T* u = static_cast<const T*>(p.u) + b * p.batch_stride;
@@ -791,7 +796,7 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         const int64_t c = c0 + col + i;
-        v[i] = col + i < cols ? to_f32<T>(p.tall ? u[c * p.row_stride + row] : u[(int64_t)row * p.row_stride + c]) : 0.f;
+        v[i] = col + i < cols ? to_f32<T>(u[(int64_t)row * p.row_stride + c]) : 0.f;
       }
     }
   };
@@ -807,6 +812,15 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
       o.w = pack_f16(v[8 * k + 6] * scale, v[8 * k + 7] * scale);
       *reinterpret_cast<uint4*>(sub + swz(row, ((col & 63) >> 3) + k)) = o;
     }
+  };
+  // ... and with what the rounding left behind it, for the m x m matrices of m <= 64 (their second sub-tile is free)
+  const bool fine = mp <= 64;
+  auto put_mat = [&](unsigned char* base, int col, float* v, float scale) {
+    put(base, col, v, scale);
+    if (!fine) return;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = v[i] * scale - __half2float(__float2half_rn(v[i] * scale));
+    put(base + C_SUB, col, v, 1.f);
   };
   // v += scale * the row's values in a matrix
   auto add = [&](const unsigned char* base, int col, float* v, float scale) {
@@ -843,17 +857,51 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
 
   // ---- x_0: raw values into tensor memory, their squares over the cluster, then scaled
   float ss = 0.f;
-  for (int g = half; g < groups; g += 4) {       // two pieces of a thread's row in flight
+  // u without 16-byte alignment, or tall: read in its own order into shared memory (the matrices' place, free until the first
+  // Gram matrix), 192 columns at a time, and the threads take their rows from there
+  constexpr int PITCH = 193;
+  float* stage = reinterpret_cast<float*>(mat);
+  const bool staged = !vec;
+  for (int g0 = 0; g0 < groups; g0 += 6) {
+  const int g1 = staged ? min(groups, g0 + 6) : groups;
+  if (staged) {
+    __syncthreads();                             // the last round has been read
+    if (p.tall) {
+      const int total = (min(cols, g1 * 32) - g0 * 32) * m;
+      const T* src = u + (int64_t)(c0 + g0 * 32) * p.row_stride;
+#pragma unroll 8
+      for (int i = threadIdx.x; i < total; i += NS_SM_THREADS) {
+        const int c = i / m, r = i - c * m;
+        stage[r * PITCH + c] = to_f32<T>(src[c * p.row_stride + r]);
+      }
+    } else {
+      for (int r = warp; r < m; r += 8) {
+        const T* src = u + (int64_t)r * p.row_stride + c0 + g0 * 32;
+#pragma unroll
+        for (int i = 0; i < 6; ++i)
+          if ((g0 + i) * 32 + lane < cols) stage[r * PITCH + i * 32 + lane] = to_f32<T>(src[i * 32 + lane]);
+      }
+    }
+    __syncthreads();
+  }
+  auto take = [&](int g, float* v) {
+    if (!staged || row >= m) { load(g * 32, v); return; }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = g * 32 + i < cols ? stage[row * PITCH + (g - g0) * 32 + i] : 0.f;
+  };
+  for (int g = g0 + half; g < g1; g += 4) {      // two pieces of a thread's row in flight
     float v[2][32];
-    load(g * 32, v[0]);
-    if (g + 2 < groups) load((g + 2) * 32, v[1]);
+    take(g, v[0]);
+    if (g + 2 < g1) take(g + 2, v[1]);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      if (g + 2 * k >= groups) break;
+      if (g + 2 * k >= g1) break;
 #pragma unroll
       for (int i = 0; i < 32; ++i) ss = fmaf(v[k][i], v[k][i], ss);
       tmem_st32(tx + lane_off + (g + 2 * k) * 32, reinterpret_cast<const uint32_t*>(v[k]));
     }
+  }
+  if (!staged) break;
   }
   tmem_st_wait();
 #pragma unroll
@@ -876,7 +924,7 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
   const float inv = 1.f / (sqrtf(ss) + p.eps);
   const float* co = p.coefficients;
   float a = p.joint ? co[0] * co[3] : co[0];
-  for (int g = half; g < groups; g += 2) {
+  for (int g = half; g < (mine ? groups : 0); g += 2) {
     float v[32];
     get(tx + g * 32, v);
 #pragma unroll
@@ -901,13 +949,13 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
     }
     wait_products();
     const float poison = *abort_flag ? __int_as_float(0x7fffffff) : 0.f;
-    for (int g = half; g < mp / 32; g += 2) {
+    for (int g = half; g < (mine ? mp / 32 : 0); g += 2) {
       float v[32];
       get(tm + g * 32, v);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = groups > 0 ? v[i] + poison : 0.f;   // an empty slice has multiplied nothing
       if (cluster == 1) {
-        put(mat, g * 32, v, 1.f / NS_ONE);
+        put_mat(mat, g * 32, v, 1.f / NS_ONE);
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -919,7 +967,8 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
       cluster_sync_all();
       tc_fence_after();
       const int quads = mp / 4;
-      for (int i = threadIdx.x; i < BM / cluster * quads; i += NS_SM_THREADS) {   // rows cta, cta + cluster, ...
+      const int my_rows = (mp - (int)cta + cluster - 1) / cluster;   // rows cta, cta + cluster, ...
+      for (int i = threadIdx.x; i < my_rows * quads; i += NS_SM_THREADS) {
         const int r = (int)cta + i / quads * cluster, k = i % quads;
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
         const float4* at = reinterpret_cast<const float4*>(exch) + r * 32 + (k ^ (r & 7));
@@ -930,9 +979,14 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
         for (int c = 0; c < cluster; ++c) { s.x += v[c].x; s.y += v[c].y; s.z += v[c].z; s.w += v[c].w; }
         const float z = 1.f / NS_ONE;
         const uint2 o = make_uint2(pack_f16(s.x * z, s.y * z), pack_f16(s.z * z, s.w * z));
+        const float2 o0 = unpack_f16(o.x), o1 = unpack_f16(o.y);
+        const uint2 rest = make_uint2(pack_f16(s.x * z - o0.x, s.y * z - o0.y), pack_f16(s.z * z - o1.x, s.w * z - o1.y));
         unsigned char* dst = mat + (k >> 4) * C_SUB + swz(r, (k & 15) >> 1) + (k & 1) * 8;
 #pragma unroll
-        for (int c = 0; c < cluster; ++c) st_remote_u2(dst, c, o);
+        for (int c = 0; c < cluster; ++c) {
+          st_remote_u2(dst, c, o);
+          if (fine) st_remote_u2(dst + C_SUB, c, rest);
+        }
       }
       fence_proxy_async_all();
       tc_fence_before();
@@ -949,20 +1003,31 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
         const uint64_t dx = make_sdesc_k128(smem_u32(mat + x * NS_MAT + (k >> 2) * C_SUB)) + (k & 3) * (32 >> 4);
         const uint64_t dy = make_sdesc_k128(smem_u32(mat + y * NS_MAT + (k >> 2) * C_SUB)) + (k & 3) * (32 >> 4);
         umma_bf16(tm, dx, dy, idesc, k != 0);
+        if (fine) {
+          umma_bf16(tm, dx, dy + (C_SUB >> 4), idesc, 1);
+          umma_bf16(tm, dx + (C_SUB >> 4), dy, idesc, 1);
+        }
       }
       umma_commit(done);
     }
     wait_products();
-    for (int g = half; g < mp / 32; g += 2) {
+    for (int g = half; g < (mine ? mp / 32 : 0); g += 2) {
       float v[32];
       get(tm + g * 32, v);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] *= alpha / NS_ONE;
       add(mat + s * NS_MAT, g * 32, v, beta);
+      if (fine) add(mat + s * NS_MAT + C_SUB, g * 32, v, beta);
       if (s2 >= 0) add(mat + s2 * NS_MAT, g * 32, v, beta2);
-      put(mat + to * NS_MAT, g * 32, v, 1.f);
+      if (s2 >= 0 && fine) add(mat + s2 * NS_MAT + C_SUB, g * 32, v, beta2);
+      put_mat(mat + to * NS_MAT, g * 32, v, 1.f);
     }
   };
+  // Results whose rows cannot be written in 16-byte pieces (all of a slice's columns) cross the matrices' place, all products being done
+  constexpr int OUT_PITCH = NS_SM_COLS + 2;
+  static_assert(BM * OUT_PITCH * 2 <= 4 * NS_MAT && BM * PITCH * 4 <= 4 * NS_MAT, "staging fits");
+  __nv_bfloat16* out_stage = reinterpret_cast<__nv_bfloat16*>(mat);
+  const bool out_vec = !p.tall && p.cols % 8 == 0 && aligned16_dev(p.out) && cols % 32 == 0;
   // x (already times a) += mat[f] x; then the next step's operand and factor, or the result
   auto apply = [&](int f, bool last, float next_a) {
     ready();
@@ -974,13 +1039,14 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
           const uint64_t df = make_sdesc_k128(smem_u32(mat + f * NS_MAT + (k >> 2) * C_SUB)) + (k & 3) * (32 >> 4);
           const uint64_t dx = make_sdesc_mn128(smem_u32(xs + (c >> 6) * C_SUB), C_SUB) + k * (2048 >> 4);
           umma_bf16(tx + c, df, dx, idesc, 1);
+          if (fine) umma_bf16(tx + c, df + (C_SUB >> 4), dx, idesc, 1);
         }
       }
       umma_commit(done);
     }
     wait_products();
     const bool failed = *abort_flag != 0;
-    for (int g = half; g < groups; g += 2) {
+    for (int g = half; g < (mine ? groups : 0); g += 2) {
       float v[32];
       get(tx + g * 32, v);
       if (!last) {
@@ -995,19 +1061,32 @@ ns_small_kernel(const __grid_constant__ NsSmallArgs p) {
       if (row >= m) continue;
       __nv_bfloat16* o = p.out + b * p.rows * p.cols;
       const int64_t c = c0 + g * 32;
-      if (!p.tall && p.cols % 8 == 0 && aligned16_dev(p.out) && g * 32 + 32 <= cols) {
+      if (out_vec && g * 32 + 32 <= cols) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           reinterpret_cast<uint4*>(o + (int64_t)row * p.cols + c)[k] =
               make_uint4(pack_bf16(v[8 * k], v[8 * k + 1]), pack_bf16(v[8 * k + 2], v[8 * k + 3]),
                          pack_bf16(v[8 * k + 4], v[8 * k + 5]), pack_bf16(v[8 * k + 6], v[8 * k + 7]));
-      } else {
+      } else {                                   // in the result's order below
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (g * 32 + i < cols) o[p.tall ? (c + i) * p.cols + row : (int64_t)row * p.cols + c + i] = __float2bfloat16_rn(v[i]);
+        for (int i = 0; i < 32; ++i) out_stage[row * OUT_PITCH + g * 32 + i] = __float2bfloat16_rn(v[i]);
       }
     }
     if (!last) tmem_st_wait();
+    if (last && !out_vec) {
+      __syncthreads();
+      __nv_bfloat16* o = p.out + b * p.rows * p.cols;
+      if (p.tall) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < cols * m; i += NS_SM_THREADS) {
+          const int c = i / m, r = i - c * m;
+          o[(int64_t)c0 * m + i] = out_stage[r * OUT_PITCH + c];
+        }
+      } else {
+        for (int r = warp; r < m; r += 8)
+          for (int c = lane; c < cols; c += 32) o[(int64_t)r * p.cols + c0 + c] = out_stage[r * OUT_PITCH + c];
+      }
+    }
   };
 
   int s = 0;
@@ -1314,9 +1393,8 @@ static int64_t ns_chunk(int64_t batch, int rows, int cols) {
 static int ns_small_cluster(int64_t batch, int rows, int cols) {
   const int m = std::min(rows, cols), n = std::max(rows, cols);
   if (m > BM || n > NS_SM_COLS * NS_SM_MAX_CLUSTER) return 0;
-  int c = 1;
-  while ((int64_t)c * NS_SM_COLS < n) c *= 2;
-  while (c < NS_SM_MAX_CLUSTER && n >= 256 * c && batch * 2 * c <= sm_count()) c *= 2;
+  int c = (n + NS_SM_COLS - 1) / NS_SM_COLS;
+  while (c < NS_SM_MAX_CLUSTER && n >= 128 * (c + 1) && batch * (c + 1) <= sm_count()) ++c;
   return c;
 }
 template <typename T, int CLUSTER>
@@ -1404,7 +1482,8 @@ extern "C" int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batc
     return dtype == BIBO_F32                                                                                                    \
                ? ns_small<float, C>(u, batch, batch_stride, rows, cols, row_stride, steps, joint, co, eps, out, st)             \
                : ns_small<__nv_bfloat16, C>(u, batch, batch_stride, rows, cols, row_stride, steps, joint, co, eps, out, st);
-  BIBO_NS_SMALL(1) BIBO_NS_SMALL(2) BIBO_NS_SMALL(4) BIBO_NS_SMALL(8)
+  BIBO_NS_SMALL(1) BIBO_NS_SMALL(2) BIBO_NS_SMALL(3) BIBO_NS_SMALL(4)
+  BIBO_NS_SMALL(5) BIBO_NS_SMALL(6) BIBO_NS_SMALL(7) BIBO_NS_SMALL(8)
 #undef BIBO_NS_SMALL
   for (int64_t b0 = 0; b0 < batch; b0 += chunk) {
     const int64_t nb = std::min(chunk, batch - b0);

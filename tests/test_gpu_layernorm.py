@@ -90,6 +90,16 @@ def test_forward_and_backward_match_the_formula(n, h, dtype, wtype):
     _compare(x, dy, w, b, 1e-5)
 
 
+@pytest.mark.parametrize("n,h", [(1185, 520), (2500, 640), (1300, 1000), (1201, 1024), (1190, 2040), (3001, 2048), (1187, 2056),
+                                 (1300, 4096), (1200, 4104), (1186, 8192), (1188, 8200)])
+@pytest.mark.parametrize("dtype,wtype,pad", [(BF, FP, 0), (BF, BF, 8), (FP, FP, 0), (FP, FP, 4)])
+def test_many_aligned_rows(n, h, dtype, wtype, pad):
+    """Rows that stream through shared memory: every width of it, the sizes around their limits, rows of a wider tensor, and
+    row counts that leave the last group short."""
+    x, dy, w, b = _inputs(n, h, dtype, wtype, True, pad, n + h)
+    _compare(x, dy, w, b, 1e-5)
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("pad", [1, 3, 4, 8, 24])
 @pytest.mark.parametrize("h", [64, 2048, 321])

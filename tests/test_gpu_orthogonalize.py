@@ -96,7 +96,8 @@ def _momentum(shape, dtype, seed, rank=8, floor=0.1, scale=1e-3):
 
 SHAPES = [(1, 1), (1, 7), (5, 1), (2, 3), (64, 64), (64, 2048), (2048, 64), (128, 128), (127, 129), (130, 257), (200, 72),
           (3, 65, 300), (2, 3, 100, 40), (4, 256, 512), (5, 512, 128), (2, 300, 900), (1, 640, 640), (2, 1030, 777),
-          (100, 384), (100, 385), (20, 100, 500), (128, 1536), (1537, 96), (7, 3000), (2500, 128), (150, 33, 129)]
+          (100, 384), (100, 385), (20, 100, 500), (128, 1536), (1537, 96), (7, 3000), (2500, 128), (150, 33, 129),
+          (12, 4000), (129, 4100), (4100, 140), (1, 256, 6000), (6, 700, 1100)]
 
 
 @pytest.mark.parametrize("shape", SHAPES)
@@ -139,6 +140,12 @@ def test_rows_and_matrices_of_larger_tensors():
         u = wide[:, :80, 1:126]
         assert torch.equal(_check(u), Fn.orthogonalize(u.contiguous()))
         assert torch.equal(Fn.orthogonalize(u[1]), Fn.orthogonalize(u.contiguous())[1])
+        tall = torch.full((3, 131, 90), float("nan"), dtype=dtype, device=DEV)
+        tall[:, 1:126, 3:83] = _momentum((3, 125, 80), dtype, 5)
+        assert torch.equal(_check(tall[:, 1:126, 3:83]), Fn.orthogonalize(tall[:, 1:126, 3:83].contiguous()))
+        large = torch.full((2, 300, 520), float("nan"), dtype=dtype, device=DEV)
+        large[:, :280, 8:408] = _momentum((2, 280, 400), dtype, 6)
+        assert torch.equal(_check(large[:, :280, 8:408]), Fn.orthogonalize(large[:, :280, 8:408].contiguous()))
         # orders that the kernels do not read: laid out first
         assert torch.equal(Fn.orthogonalize(u.mT), Fn.orthogonalize(u.mT.contiguous()))
         assert torch.equal(Fn.orthogonalize(u[0].expand(2, -1, -1)), Fn.orthogonalize(u[:1].repeat(2, 1, 1)))
@@ -195,6 +202,23 @@ def test_two_graphs_and_streams_do_not_share_a_workspace():
     a.copy_(new)
     graphs[0][0].replay()
     assert torch.equal(graphs[0][1], Fn.orthogonalize(new))
+
+
+def test_calls_on_two_streams_at_once():
+    from bibo_b200 import functional as Fn
+    us = [_momentum(shape, torch.bfloat16, 7 + i) for i, shape in enumerate([(1, 520, 600), (4, 300, 700), (3, 64, 900), (1, 200, 3400)])]
+    want = [Fn.orthogonalize(u) for u in us]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for s, out in zip(streams, got):
+            with torch.cuda.stream(s):
+                out.append([Fn.orthogonalize(u) for u in us])
+    torch.cuda.synchronize()
+    for out in got:
+        for run in out:
+            assert all(torch.equal(a, b) for a, b in zip(run, want))
 
 
 def test_muon_step_on_the_blocks_parameters():
