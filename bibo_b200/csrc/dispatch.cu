@@ -215,10 +215,8 @@ dispatch_rows_kernel(const I* __restrict__ idx, int64_t slots, int64_t per_block
   int32_t* slot_row = plan + dp_off_slot_row(E);
   int32_t* row_slot = plan + dp_off_row_slot(E, slots);
   if (b == 0) {
-    int bad = 0;
-    if (threadIdx.x == 0)
-      for (int i = 0; i < n; ++i) bad |= scratch[(int64_t)n * E + i];
-    dp_write_head(d, E, bad, plan);
+    // n <= DP_MAX_BLOCKS flags
+    dp_write_head(d, E, __syncthreads_or((int)threadIdx.x < n ? scratch[(int64_t)n * E + threadIdx.x] : 0), plan);
   }
   dp_free_rows(d, E, align, rows_cap, b, n, row_slot);
   const int64_t s0 = min(slots, b * per_block), s1 = min(slots, s0 + per_block);

@@ -118,6 +118,29 @@ def test_plan_at_the_block_and_cluster_sizes(n, k, e):
     _check_plan(Fn.dispatch_plan(same.to(DEV), e, 128), same, e, 128)
 
 
+def test_offsets_beyond_32_bits():
+    """Expert-ordered rows of more than 2^31 elements (and 2^32 bytes): the last rows are where they should be."""
+    from bibo_b200 import functional as Fn
+    n, k, e, h = 34000, 8, 16, 8192
+    idx = torch.arange(k, device=DEV, dtype=torch.int32).expand(n, k) * 2
+    plan = Fn.dispatch_plan(idx.contiguous(), e)
+    assert plan.rows * h > 1 << 31
+    x = torch.randn(n, h, device=DEV).to(BF)
+    xs = Fn.dispatch_forward(x, plan)
+    for j in (0, k - 1):                                           # expert 2j holds all tokens in order
+        assert torch.equal(xs[j * n:(j + 1) * n], x)
+    w = torch.rand(n, k, device=DEV)
+    out = Fn.combine_forward(xs, w, plan)
+    t = torch.tensor([0, 1, n // 2, n - 1], device=DEV)
+    want = x[t].double() * w[t].double().sum(1, keepdim=True)
+    assert bool(((out[t].double() - want).abs() <= ((k + 1) * U + 1.01 * _half(BF)) * want.abs()).all())
+    dys, dw = Fn.combine_backward(x, xs, w, plan)
+    want = w[t, k - 1].double()[:, None] * x[t].double()
+    assert bool(((dys[(k - 1) * n + t].double() - want).abs() <= 1.01 * (_half(BF) + U) * want.abs()).all())
+    sq = x[t].double().square().sum(1)
+    assert bool(((dw[t, k - 1].double() - sq).abs() <= (h / 32 + 16) * U * sq).all())
+
+
 def test_no_tokens_and_out_of_range_indices():
     from bibo_b200 import functional as Fn
     plan = Fn.dispatch_plan(torch.empty(0, 4, dtype=torch.int64, device=DEV), 8, 16)

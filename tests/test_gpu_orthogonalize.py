@@ -290,7 +290,7 @@ def test_training_step_with_the_callers_own_experts():
     (outd * c.double()).sum().backward()
     # fp32 throughout (the experts' products are torch's): sums of at most 150 x 64 order-1 terms, 1e-4 of the largest entry
     for got, want in ((norm.weight.grad, p["nw"].grad), (norm.bias.grad, p["nb"].grad), (w1.grad, p["w1"].grad),
-                      (w2.grad, p["w2"].grad), (weight.grad, p["weight"].grad), (out, outd.detach())):
+                      (w2.grad, p["w2"].grad), (weight.grad, p["weight"].grad), (out.detach(), outd.detach())):
         assert float((got.double() - want).abs().max()) <= 1e-4 * float(want.abs().max())
     for q in (w1, w2):
         _check(q.grad)
