@@ -7,7 +7,7 @@
 // Numbers.  The products run on the tensor cores with f16 operands and fp32 accumulators: bf16 operands would lose
 // three bits more, tf32 would halve the rate for none, and the range is bounded (|x|_2 <= about 1.2 for the usual
 // coefficients, so every entry of x, G and b G + c G^2 is below 16).  All three are kept times 2^12, which centres
-// them in f16's range: an entry 2^-26 of the largest is still normal.  u enters scaled by a power of two (exact for bf16)
+// them in f16's range: an entry of 2^-26 is still a normal number.  u enters scaled by a power of two (exact for bf16)
 // and the rest of 1/(|u|_F + eps), t in [1,2), goes into the first products' epilogues in fp32.
 // A rounding of x spreads over all singular directions, and a direction of a small singular value is stretched by
 // a ~ 3.4 in every step that follows, so the early x are what has to be exact:
@@ -571,16 +571,14 @@ template <int MODE> __device__ __forceinline__ NsTile ns_decode_single(int64_t w
   return t;
 }
 template <int OP>
-__device__ __forceinline__ bool ns_load_single(unsigned char* dst, const NsMaps& m, uint64_t* bar, int tile, int kb, int b) {
+__device__ __forceinline__ void ns_load_single(unsigned char* dst, const NsMaps& m, uint64_t* bar, int tile, int kb, int b) {
   const int r0 = tile * BM;
-  const bool mn = OP == OP_MN || (OP == OP_SYM && kb / (BM / BK) > tile);
-  if (mn) {
+  if (OP == OP_MN || (OP == OP_SYM && kb / (BM / BK) > tile)) {
     tma_load_3d(dst, &m.r64, bar, r0, kb * BK, b);
     tma_load_3d(dst + MN_BOX, &m.r64, bar, r0 + 64, kb * BK, b);
   } else {
     tma_load_3d(dst, &m.r128, bar, kb * BK, r0, b);
   }
-  return mn;
 }
 template <int MODE, bool TALL>
 __global__ void __launch_bounds__(NS_THREADS, 1)

@@ -611,14 +611,25 @@ def _rows_like(t: torch.Tensor, name: str, n: int, h: int, like: torch.Tensor) -
 
 def _launch(name: str, dev: torch.device, *args) -> None:
     """One C-ABI call on ``dev``'s current stream, with ``dev`` made current for it where another device is."""
-    fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, _raw_stream(dev.index))
+    fn = _entry(name)
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev.index))
+            rc = fn(*args, _raw_stream(index))
     if rc != 0:
         _lib.check(rc, name)
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    return getattr(_lib.load(), name)
+
+
+@functools.lru_cache(maxsize=1024)
+def _layernorm_parts(n: int) -> int:
+    return int(_lib.load().bibo_moe_layernorm_bwd_parts(n))
 
 
 # the current stream as an address: a tenth of the time of building a Stream object for it
@@ -631,20 +642,22 @@ def layernorm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bi
     fp32 and rounded once.  The rows may be a slice of a wider tensor.  ``weight`` and ``bias`` [H] are each optional and
     share one dtype, fp32 or that of x.  ``keep=True`` returns ``(out, saved)`` with what ``layernorm_backward`` needs."""
     n, hidden, stride = _rows(x, "x")
-    wtype = dtype = x.dtype
+    dev, wtype = x.device, x.dtype
+    dtype = wtype
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
         _need_cuda(t, name)
-        if t.shape != (hidden,) or t.device != x.device:
-            raise RuntimeError(f"{name} must be [{hidden}] on {x.device}, got {tuple(t.shape)} on {t.device}")
-        if t.dtype not in (dtype, torch.float32) or (t is bias and weight is not None and bias.dtype != weight.dtype):
-            raise RuntimeError(f"{name} dtype {t.dtype}: weight and bias are both float32 or both {dtype}")
-        wtype = t.dtype
+        if t.dim() != 1 or t.shape[0] != hidden or t.device != dev:
+            raise RuntimeError(f"{name} must be [{hidden}] on {dev}, got {tuple(t.shape)} on {t.device}")
+        tt = t.dtype
+        if (tt != dtype and tt != torch.float32) or (t is bias and weight is not None and tt != wtype):
+            raise RuntimeError(f"{name} dtype {tt}: weight and bias are both float32 or both {dtype}")
+        wtype = tt
     out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    stats = torch.empty((2, n), dtype=torch.float32, device=x.device) if keep else None
+    stats = torch.empty((2, n), dtype=torch.float32, device=dev) if keep else None
     mean = None if stats is None else stats.data_ptr()
-    _launch("bibo_moe_layernorm_fwd", x.device, x.data_ptr(), stride, None if weight is None else weight.data_ptr(),
+    _launch("bibo_moe_layernorm_fwd", dev, x.data_ptr(), stride, None if weight is None else weight.data_ptr(),
             None if bias is None else bias.data_ptr(), eps, n, hidden, dtype_code(dtype), dtype_code(wtype), out.data_ptr(), mean,
             None if stats is None else mean + 4 * n)
     return (out, (stats, wtype)) if keep else out
@@ -666,8 +679,7 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch
     dbias = make(hidden, dtype=wtype, device=dev) if has_bias else None
     partial = None
     if dweight is not None or dbias is not None:
-        parts = int(_lib.load().bibo_moe_layernorm_bwd_parts(n))
-        partial = torch.empty((parts, 2, hidden), dtype=torch.float32, device=dev)
+        partial = torch.empty((_layernorm_parts(n), 2, hidden), dtype=torch.float32, device=dev)
     p = _lib.ptr
     _launch("bibo_moe_layernorm_bwd", dev, p(x), stride, p(dy), dy_stride, p(weight), p(stats), p(stats) + 4 * n, n,
             hidden, dtype_code(x.dtype), dtype_code(wtype), p(dx), p(partial), p(dweight), p(dbias))
