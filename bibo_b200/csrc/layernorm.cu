@@ -190,7 +190,8 @@ template <typename T, typename W, int VE, int NT, int CH, int R>
 __global__ void __launch_bounds__(NT)
 layernorm_bwd_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ dy, int64_t dy_stride,
                      const W* __restrict__ weight, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
-                     int64_t n_rows, int hidden, T* __restrict__ dx, float* __restrict__ partial) {
+                     int64_t n_rows, int hidden, T* __restrict__ dx, float* __restrict__ partial, W* __restrict__ dweight,
+                     W* __restrict__ dbias) {
   using X = LnVec<T, VE>;
   using V = typename X::V;
   constexpr int WARPS = NT / 32;
@@ -282,6 +283,19 @@ layernorm_bwd_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restr
         ds[c] = X::pack(f);
       }
     }
+  }
+  if (gridDim.x == 1) {                          // the only block: its sums are the gradients
+#pragma unroll
+    for (int q = 0; q < CH; ++q) {
+      const int c = q * NT + tid;
+      if (c >= vecs) continue;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        if (dweight != nullptr) dweight[c * VE + i] = from_f32<W>(dw[q][i]);
+        if (dbias != nullptr) dbias[c * VE + i] = from_f32<W>(db[q][i]);
+      }
+    }
+    return;
   }
   if (partial == nullptr) return;
   float* p = partial + (int64_t)blockIdx.x * 2 * hidden;
@@ -442,7 +456,8 @@ template <typename T, typename W, int NT, int CH, int R>
 __global__ void __launch_bounds__(NT)
 layernorm_bwd_ring_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ dy, int64_t dy_stride,
                           const W* __restrict__ weight, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
-                          int64_t n_rows, int hidden, int stages, T* __restrict__ dx, float* __restrict__ partial) {
+                          int64_t n_rows, int hidden, int stages, T* __restrict__ dx, float* __restrict__ partial, W* __restrict__ dweight,
+                     W* __restrict__ dbias) {
   constexpr int VE = 16 / sizeof(T), P = VE / 2, WARPS = NT / 32;
   using X = LnVec<T, VE>;
   extern __shared__ __align__(16) unsigned char ring[];          // [stages][R][x row, dy row]
@@ -557,7 +572,18 @@ layernorm_bwd_ring_kernel(const T* __restrict__ x, int64_t x_stride, const T* __
     }
     if (++st == stages) { st = 0; phase ^= 1; }
   }
-  if (partial != nullptr) {
+  if (gridDim.x == 1) {                          // the only block: its sums are the gradients
+#pragma unroll
+    for (int q = 0; q < CH; ++q) {
+      const int c = (q * NT + tid) * VE;
+      if (c >= hidden) continue;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        if (dweight != nullptr) dweight[c + i] = from_f32<W>(i & 1 ? dw[q][i / 2].y : dw[q][i / 2].x);
+        if (dbias != nullptr) dbias[c + i] = from_f32<W>(i & 1 ? db[q][i / 2].y : db[q][i / 2].x);
+      }
+    }
+  } else if (partial != nullptr) {
     float* p = partial + (int64_t)blockIdx.x * 2 * hidden;
 #pragma unroll
     for (int q = 0; q < CH; ++q) {
@@ -575,7 +601,8 @@ layernorm_bwd_ring_kernel(const T* __restrict__ x, int64_t x_stride, const T* __
 }
 
 constexpr int LN_MAX_PARTS = 592;
-static int64_t ln_parts(int64_t n_rows) { return n_rows < LN_MAX_PARTS ? n_rows : LN_MAX_PARTS; }
+constexpr int LN_ONE_BLOCK = 16;     // up to as many rows one block takes all, without partial sums and their launch
+static int64_t ln_parts(int64_t n_rows) { return n_rows <= LN_ONE_BLOCK ? 0 : n_rows < LN_MAX_PARTS ? n_rows : LN_MAX_PARTS; }
 
 // the widest access that rows of `hidden` elements of `size` bytes allow at these addresses; strides in elements (0: one row)
 static int ln_access(int hidden, int size, int wsize, int64_t s0, int64_t s1, const void* a, const void* b, const void* c, const void* w,
@@ -654,11 +681,11 @@ layernorm_bwd_dx_loop_kernel(const T* __restrict__ x, int64_t x_stride, const T*
 }
 
 // dw / db of one range of rows per block row: a thread per column, rows in ascending order
-template <typename T>
+template <typename T, typename W>
 __global__ void __launch_bounds__(LN_T)
 layernorm_bwd_cols_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ dy, int64_t dy_stride,
                           const float* __restrict__ mean_in, const float* __restrict__ rstd_in, int64_t n_rows, int hidden,
-                          int64_t rows_per_part, float* __restrict__ partial) {
+                          int64_t rows_per_part, float* __restrict__ partial, W* __restrict__ dweight, W* __restrict__ dbias) {
   const int c = blockIdx.y * LN_T + threadIdx.x;
   if (c >= hidden) return;
   const int64_t r0 = blockIdx.x * rows_per_part, r1 = r0 + rows_per_part < n_rows ? r0 + rows_per_part : n_rows;
@@ -667,6 +694,11 @@ layernorm_bwd_cols_kernel(const T* __restrict__ x, int64_t x_stride, const T* __
     const float g = to_f32<T>(dy[r * dy_stride + c]);
     db += g;
     dw = fmaf(g, (to_f32<T>(x[r * x_stride + c]) - mean_in[r]) * rstd_in[r], dw);
+  }
+  if (gridDim.x == 1) {
+    if (dweight != nullptr) dweight[c] = from_f32<W>(dw);
+    if (dbias != nullptr) dbias[c] = from_f32<W>(db);
+    return;
   }
   float* p = partial + (int64_t)blockIdx.x * 2 * hidden;
   p[c] = dw;
@@ -785,7 +817,7 @@ static int layernorm_fwd_t(const void* x, int64_t x_stride, const void* weight, 
 template <typename T, typename W, int VE, int NT, int CH, int R>
 static int layernorm_bwd_v(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
                            const float* mean, const float* rstd, int64_t n_rows, int hidden, void* dx, float* partial,
-                           int* parts, cudaStream_t st) {
+                           void* dweight, void* dbias, int* parts, cudaStream_t st) {
   auto kern = layernorm_bwd_kernel<T, W, VE, NT, CH, R>;
   static DeviceOnce once;
   int per_sm = 1;
@@ -794,12 +826,13 @@ static int layernorm_bwd_v(const void* x, int64_t x_stride, const void* dy, int6
     return (int)BIBO_OK;
   }, &per_sm);
   if (rc) return rc;
-  int64_t grid = (n_rows + R - 1) / R;
+  int64_t grid = n_rows <= LN_ONE_BLOCK ? 1 : (n_rows + R - 1) / R;
   const int64_t fit = (int64_t)sm_count() * (per_sm > 0 ? per_sm : 1);
   if (grid > fit) grid = fit;
   if (grid > LN_MAX_PARTS) grid = LN_MAX_PARTS;
   kern<<<(unsigned)grid, NT, 0, st>>>(static_cast<const T*>(x), x_stride, static_cast<const T*>(dy), dy_stride,
-                                      static_cast<const W*>(weight), mean, rstd, n_rows, hidden, static_cast<T*>(dx), partial);
+                                      static_cast<const W*>(weight), mean, rstd, n_rows, hidden, static_cast<T*>(dx), partial,
+                                      static_cast<W*>(dweight), static_cast<W*>(dbias));
   BIBO_CHECK_LAUNCH("layernorm_bwd_kernel");
   *parts = (int)grid;
   return BIBO_OK;
@@ -808,7 +841,7 @@ static int layernorm_bwd_v(const void* x, int64_t x_stride, const void* dy, int6
 template <typename T, typename W, int NT, int CH, int R, int CTAS>
 static int layernorm_bwd_ring(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
                               const float* mean, const float* rstd, int64_t n_rows, int hidden, void* dx, float* partial,
-                              int* parts, cudaStream_t st) {
+                              void* dweight, void* dbias, int* parts, cudaStream_t st) {
   auto kern = layernorm_bwd_ring_kernel<T, W, NT, CH, R>;
   constexpr int RING = 208 * 1024 / CTAS;        // CTAS blocks share an SM
   static DeviceOnce once;
@@ -820,14 +853,14 @@ static int layernorm_bwd_ring(const void* x, int64_t x_stride, const void* dy, i
   }, &per_sm);
   if (rc) return rc;
   const int group = R * 2 * hidden * (int)sizeof(T);
-  int64_t grid = (n_rows + R - 1) / R;
+  int64_t grid = n_rows <= LN_ONE_BLOCK ? 1 : (n_rows + R - 1) / R;
   if (grid > per_sm * (int64_t)sm_count()) grid = per_sm * (int64_t)sm_count();
   if (grid > LN_MAX_PARTS) grid = LN_MAX_PARTS;
   int stages = RING / group;
   if (stages > LN_MAX_STAGES) stages = LN_MAX_STAGES;
   kern<<<(unsigned)grid, NT, stages * group, st>>>(static_cast<const T*>(x), x_stride, static_cast<const T*>(dy), dy_stride,
                                                    static_cast<const W*>(weight), mean, rstd, n_rows, hidden, stages,
-                                                   static_cast<T*>(dx), partial);
+                                                   static_cast<T*>(dx), partial, static_cast<W*>(dweight), static_cast<W*>(dbias));
   BIBO_CHECK_LAUNCH("layernorm_bwd_ring_kernel");
   *parts = (int)grid;
   return BIBO_OK;
@@ -837,7 +870,7 @@ static int layernorm_bwd_ring(const void* x, int64_t x_stride, const void* dy, i
 template <typename T, typename W, int VE>
 static int layernorm_bwd_pick(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
                               const float* mean, const float* rstd, int64_t n_rows, int hidden, void* dx, float* partial,
-                              int* parts, bool* done, cudaStream_t st) {
+                              void* dweight, void* dbias, int* parts, bool* done, cudaStream_t st) {
   const int vecs = hidden / VE;
   *done = true;
   if constexpr (VE * sizeof(T) == 16) {
@@ -845,7 +878,7 @@ static int layernorm_bwd_pick(const void* x, int64_t x_stride, const void* dy, i
     // threads, pieces a thread, rows a group, blocks an SM.  bf16 rows with fp32 weight, measured: 32768 x 2048 73 us (0.84 of the
     // copy rate; two rows a group: 79, 128 threads of 16 columns: 79), 32768 x 1024 46 us (0.67), 16384 x 4096 77 us (0.80).
 #define BIBO_LN_RING(...)                                                                                                     \
-  return layernorm_bwd_ring<T, W, __VA_ARGS__>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, partial, parts, st)
+  return layernorm_bwd_ring<T, W, __VA_ARGS__>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, partial, dweight, dbias, parts, st)
     if (hidden > 512 && hidden <= 1024) BIBO_LN_RING(128, C8, 4, 4);
     if (hidden > 1024 && hidden <= 2048) BIBO_LN_RING(256, C8, 4, 2);
     if (hidden > 2048 && hidden <= 4096) BIBO_LN_RING(256, C16, 1, 2);
@@ -853,7 +886,7 @@ static int layernorm_bwd_pick(const void* x, int64_t x_stride, const void* dy, i
 #undef BIBO_LN_RING
   }
 #define BIBO_LN_BWD(NT, CH, R)                                                                                              \
-  return layernorm_bwd_v<T, W, VE, NT, CH, R>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, partial, parts, st)
+  return layernorm_bwd_v<T, W, VE, NT, CH, R>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, partial, dweight, dbias, parts, st)
   if (vecs <= 64) BIBO_LN_BWD(64, 1, 8);
   if (vecs <= 128) BIBO_LN_BWD(128, 1, 4);
   if (vecs <= 256) BIBO_LN_BWD(256, 1, 4);
@@ -878,7 +911,7 @@ static int layernorm_bwd_t(const void* x, int64_t x_stride, const void* dy, int6
   int used = 0, rc = BIBO_OK;
   bool done = false;
   float* part = params ? partial : nullptr;
-#define BIBO_LN_PICK(VE) layernorm_bwd_pick<T, W, VE>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, part, &used, &done, st)
+#define BIBO_LN_PICK(VE) layernorm_bwd_pick<T, W, VE>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, part, dweight, dbias, &used, &done, st)
   if constexpr (sizeof(T) == 2) rc = ve == 8 ? BIBO_LN_PICK(8) : ve == 2 ? BIBO_LN_PICK(2) : BIBO_LN_PICK(1);
   else rc = ve == 4 ? BIBO_LN_PICK(4) : BIBO_LN_PICK(1);
 #undef BIBO_LN_PICK
@@ -889,13 +922,14 @@ static int layernorm_bwd_t(const void* x, int64_t x_stride, const void* dy, int6
         hidden, static_cast<T*>(dx));
     BIBO_CHECK_LAUNCH("layernorm_bwd_dx_loop_kernel");
     if (!params) return BIBO_OK;
-    const int64_t parts = ln_parts(n_rows), per = (n_rows + parts - 1) / parts;
+    const int64_t parts = n_rows <= LN_ONE_BLOCK ? 1 : ln_parts(n_rows), per = (n_rows + parts - 1) / parts;
     used = (int)((n_rows + per - 1) / per);
-    layernorm_bwd_cols_kernel<T><<<dim3(used, (hidden + LN_T - 1) / LN_T), LN_T, 0, st>>>(
-        static_cast<const T*>(x), x_stride, static_cast<const T*>(dy), dy_stride, mean, rstd, n_rows, hidden, per, partial);
+    layernorm_bwd_cols_kernel<T, W><<<dim3(used, (hidden + LN_T - 1) / LN_T), LN_T, 0, st>>>(
+        static_cast<const T*>(x), x_stride, static_cast<const T*>(dy), dy_stride, mean, rstd, n_rows, hidden, per, partial,
+        static_cast<W*>(dweight), static_cast<W*>(dbias));
     BIBO_CHECK_LAUNCH("layernorm_bwd_cols_kernel");
   }
-  if (!params) return BIBO_OK;
+  if (!params || used == 1) return BIBO_OK;      // one block has written the gradients itself
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((hidden + 31) / 32, 2);
   cfg.blockDim = dim3(1024);
@@ -949,7 +983,7 @@ extern "C" int bibo_moe_layernorm_bwd(const void* x, int64_t x_stride, const voi
   if (!rc) rc = layernorm_check("layernorm_bwd", n_rows, hidden, dtype, wdtype, n_rows > 1 ? dy_stride : hidden);
   if (rc) return rc;
   if (n_rows <= 0) return BIBO_OK;      // the caller's dweight / dbias are sums over no rows: it zeroes them itself
-  if (!x || !dy || !mean || !rstd || !dx || ((dweight || dbias) && !partial))
+  if (!x || !dy || !mean || !rstd || !dx || ((dweight || dbias) && !partial && ln_parts(n_rows) > 0))
     return fail(BIBO_ERR_ARG, "layernorm_bwd: null pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == BIBO_F32)

@@ -443,10 +443,11 @@ class DispatchPlan:
     * ``row_slot`` int32 [rows]: slot ``t*k + j`` of a row, -1 for a row without one
     """
 
-    def __init__(self, n_tokens: int, top_k: int, n_experts: int, align: int, device):
+    def __init__(self, n_tokens: int, top_k: int, n_experts: int, align: int, device, like: Optional[torch.Tensor] = None):
         self.n_tokens, self.top_k, self.n_experts, self.align = n_tokens, top_k, n_experts, align
         self.rows, words, self._slot_row, self._row_slot = _plan_layout(n_tokens, top_k, n_experts, align)
-        self.buf = torch.empty(words, dtype=torch.int32, device=device)
+        self.buf = (torch.empty(words, dtype=torch.int32, device=device) if like is None
+                    else like.new_empty(words, dtype=torch.int32))
 
     @property
     def offsets(self) -> torch.Tensor:
@@ -480,7 +481,7 @@ def dispatch_plan(topk_idx: torch.Tensor, n_experts: int, align: int = 1) -> Dis
         raise RuntimeError(f"topk_idx must be int32 or int64 [N, k], got {topk_idx.dtype} {tuple(topk_idx.shape)}")
     n, k = topk_idx.shape
     dev = topk_idx.device
-    plan = DispatchPlan(n, k, int(n_experts), int(align), dev)
+    plan = DispatchPlan(n, k, int(n_experts), int(align), dev, topk_idx)
     _launch("bibo_moe_dispatch_plan", dev, topk_idx.data_ptr(), topk_idx.element_size(), n, k, plan.n_experts, plan.align,
             plan.buf.data_ptr())
     return plan
@@ -655,7 +656,7 @@ def layernorm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bi
             raise RuntimeError(f"{name} dtype {tt}: weight and bias are both float32 or both {dtype}")
         wtype = tt
     out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    stats = torch.empty((2, n), dtype=torch.float32, device=dev) if keep else None
+    stats = x.new_empty((2, n), dtype=torch.float32) if keep else None
     mean = None if stats is None else stats.data_ptr()
     _launch("bibo_moe_layernorm_fwd", dev, x.data_ptr(), stride, None if weight is None else weight.data_ptr(),
             None if bias is None else bias.data_ptr(), eps, n, hidden, dtype_code(dtype), dtype_code(wtype), out.data_ptr(), mean,
@@ -674,12 +675,11 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch
         raise RuntimeError(f"the forward kept {stats.shape[1]} rows, x has {n}")
     dev = x.device
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-    make = torch.empty if n else torch.zeros                   # sums over no rows
-    dweight = make(hidden, dtype=wtype, device=dev) if weight is not None and need_dweight else None
-    dbias = make(hidden, dtype=wtype, device=dev) if has_bias else None
-    partial = None
-    if dweight is not None or dbias is not None:
-        partial = torch.empty((_layernorm_parts(n), 2, hidden), dtype=torch.float32, device=dev)
+    make = x.new_empty if n else x.new_zeros                   # sums over no rows
+    dweight = make(hidden, dtype=wtype) if weight is not None and need_dweight else None
+    dbias = make(hidden, dtype=wtype) if has_bias else None
+    parts = _layernorm_parts(n) if dweight is not None or dbias is not None else 0
+    partial = x.new_empty((parts, 2, hidden), dtype=torch.float32) if parts else None
     p = _lib.ptr
     _launch("bibo_moe_layernorm_bwd", dev, p(x), stride, p(dy), dy_stride, p(weight), p(stats), p(stats) + 4 * n, n,
             hidden, dtype_code(x.dtype), dtype_code(wtype), p(dx), p(partial), p(dweight), p(dbias))

@@ -556,7 +556,8 @@ int bibo_moe_layernorm_fwd(const void* x, int64_t x_stride, const void* weight, 
                            int64_t n_rows, int hidden, int dtype, int wdtype, void* out, float* mean, float* rstd,
                            void* stream);
 /* dx [N,H] contiguous, dweight / dbias [H] in wdtype (either NULL: not wanted); partial is fp32 scratch
- * [bibo_moe_layernorm_bwd_parts(N), 2, H].  Deterministic (no float atomics).  n_rows == 0 writes nothing. */
+ * [bibo_moe_layernorm_bwd_parts(N), 2, H] (NULL where that is 0).  Deterministic (no float atomics).  n_rows == 0
+ * writes nothing.                                                                                        */
 int64_t bibo_moe_layernorm_bwd_parts(int64_t n_rows);
 int bibo_moe_layernorm_bwd(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
                            const float* mean, const float* rstd, int64_t n_rows, int hidden, int dtype, int wdtype,
