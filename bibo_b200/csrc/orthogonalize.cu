@@ -1293,8 +1293,10 @@ template <int MODE, bool TALL> static int ns_launch(NsArgs& p, int64_t batch, in
   p.k_blocks = (k_dim + BK - 1) / BK;
   p.n_work = batch * (MODE == NS_APPLY ? (int64_t)p.m_tiles * p.n_tiles : (int64_t)p.m_tiles * (p.m_tiles + 1) / 2);
   p.batch = batch;
-  // 128 x 128 tiles that fit the machine at once, unless k is so long that splitting it over pairs gains more than the exchange
-  // costs.  All steps of 1024 x 1024: 151 us this way, 186 split, 218 with a pair per tile; of 512 x 8192: 249 us against 198.
+  // 128 x 128 tiles where they need no more waves than the pairs' tiles (up to two: beyond that the pairs' drain under the next
+  // tile's products wins), unless k is so long that splitting it over pairs gains more than the exchange costs.  A wave takes
+  // about the same either way, a CTA of both kernels loads 32 KB per k-block.  All steps of 1024 x 1024: 151 us this way, 186
+  // split, 218 with a pair per tile; of 512 x 8192: 249 us against 198 split.
   if (p.k_blocks <= 40) {
     const int mt = (p.rows + BM - 1) / BM, nt = (p.cols + NS_ST_BN - 1) / NS_ST_BN;
     int64_t tiles = (int64_t)mt * nt;
@@ -1302,7 +1304,8 @@ template <int MODE, bool TALL> static int ns_launch(NsArgs& p, int64_t batch, in
       tiles = 0;
       for (int i = 0; i < mt; ++i) tiles += std::min(i / 2 * 2 + 2, mt);
     }
-    if (batch * tiles <= sm_count()) {
+    const int64_t sms = sm_count(), waves = (batch * tiles + sms - 1) / sms;
+    if (waves <= 2 && waves <= (p.n_work + sms / 2 - 1) / (sms / 2)) {
       NsArgs q = p;
       q.m_tiles = mt;
       q.n_tiles = nt;
