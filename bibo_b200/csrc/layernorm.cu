@@ -797,7 +797,7 @@ static int layernorm_fwd_t(const void* x, int64_t x_stride, const void* weight, 
   // (0.86 of the copy rate; 256 threads of 8 columns: 56.6), 32768 x 1024 25.5 us (0.80; 128 threads of 8: 31.9), 16384 x 4096 48 us.
   // Below eight rows an SM a ring has nothing to run ahead of.
   if (ve * sizeof(T) == 16 && n_rows > 8 * (int64_t)sm_count()) {
-    constexpr int VE = 16 / sizeof(T), C8 = 8 / VE, C16 = 16 / VE;    // pieces of 16 bytes for 8 and 16 columns a thread
+    constexpr int VE = 16 / sizeof(T), C16 = 16 / VE;                 // pieces of 16 bytes for 16 columns a thread
 #define BIBO_LN_RING(...) return layernorm_fwd_ring<T, W, __VA_ARGS__>(x, x_stride, weight, bias, eps, n_rows, hidden, out, mean, rstd, st)
     if (hidden > 512 && hidden <= 1024) BIBO_LN_RING(64, C16, 4, 8);
     if (hidden > 1024 && hidden <= 2048) BIBO_LN_RING(128, C16, 4, 3);
