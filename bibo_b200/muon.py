@@ -33,6 +33,14 @@ class Muon(torch.optim.Optimizer):
                 if p.dim() < 2:
                     raise ValueError(f"Muon takes matrices and stacks of them, got a parameter of shape {tuple(p.shape)}")
 
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        keys = [k for group in state_dict["param_groups"] for k in group["params"]]
+        for key, p in zip(keys, [p for group in self.param_groups for p in group["params"]]):
+            buf = state_dict["state"].get(key, {}).get("momentum_buffer")
+            if buf is not None:                     # torch casts a state to the parameter's type; the momentum stays in fp32
+                self.state[p]["momentum_buffer"] = buf.to(device=p.device, dtype=torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -42,10 +50,12 @@ class Muon(torch.optim.Optimizer):
         for group in self.param_groups:
             momentum = group["momentum"]
             for p in group["params"]:
-                if p.grad is None:
+                if p.grad is None or p.numel() == 0:
                     continue
                 state = self.state[p]
                 if "momentum_buffer" not in state:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():   # every replay would clear the momentum
+                        raise RuntimeError("Muon: take a step, or load a state, before a step is captured in a graph")
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 buf = state["momentum_buffer"]
                 buf.mul_(momentum).add_(p.grad)

@@ -302,3 +302,29 @@ def test_training_step_with_the_callers_own_experts():
     want, bound = _steps64(w1.grad.float(), 5, NS)
     size = want.flatten(-2).norm(dim=-1)
     assert bool(((step - want).flatten(-2).norm(dim=-1) <= 4 * bound + (2.0 ** -8 + 1e-4) * size).all())
+
+
+def test_muon_refuses_to_capture_its_first_step():
+    import bibo_b200
+    p = torch.nn.Parameter(torch.randn(64, 96, device=DEV))
+    p.grad = torch.randn_like(p)
+    opt = bibo_b200.Muon([p])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="before a step is captured"):
+            opt.step()
+        unused = p.detach() + 1                                        # the capture itself is whole
+    opt.step()
+    start, buf = p.detach().clone(), opt.state[p]["momentum_buffer"].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(2):
+        graph.replay()
+    got, got_buf = p.detach().clone(), opt.state[p]["momentum_buffer"].clone()
+    with torch.no_grad():
+        p.copy_(start)
+        opt.state[p]["momentum_buffer"].copy_(buf)
+    for _ in range(2):
+        opt.step()
+    assert torch.equal(got, p.detach()) and torch.equal(got_buf, opt.state[p]["momentum_buffer"])

@@ -177,3 +177,23 @@ def test_orthogonalize_refusals_and_workspace():
         bibo_b200.Muon([torch.nn.Parameter(torch.zeros(4))])
     with pytest.raises(ValueError, match="momentum"):
         bibo_b200.Muon([torch.nn.Parameter(torch.zeros(4, 4))], momentum=1.0)
+
+
+def test_muon_state_loads_in_fp32():
+    import bibo_b200
+    make = lambda: bibo_b200.Muon([torch.nn.Parameter(torch.zeros(4, 6, dtype=t)) for t in (torch.bfloat16, torch.float32)])
+    a, b = make(), make()
+    for p in a.param_groups[0]["params"]:
+        a.state[p]["momentum_buffer"] = torch.randn(4, 6)
+    b.load_state_dict(a.state_dict())
+    for p, q in zip(a.param_groups[0]["params"], b.param_groups[0]["params"]):
+        got, want = b.state[q]["momentum_buffer"], a.state[p]["momentum_buffer"]
+        assert got.dtype == torch.float32 and torch.equal(got, want) and got.data_ptr() != want.data_ptr()
+    make().load_state_dict(make().state_dict())                        # no step taken yet
+
+
+def test_muon_skips_empty_parameters():
+    import bibo_b200
+    p = torch.nn.Parameter(torch.zeros(4, 0))
+    p.grad = torch.zeros(4, 0)
+    bibo_b200.Muon([p]).step()
