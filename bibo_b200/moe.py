@@ -348,11 +348,16 @@ def ffn_forward(decoder_layer, hidden_states: torch.Tensor) -> torch.Tensor:
     into the combine kernel; with gradients on, norm and block run through their autograd nodes (kernels
     in both directions) and the residual add is torch's.  Written against the reference's attribute
     names (``post_attention_layernorm``, ``mlp``, ``_bf16_moe_out``, ``_bf16_stream``).  A norm that is a
-    ``torch.nn.LayerNorm`` runs on the layer norm kernels, in both directions."""
+    ``torch.nn.LayerNorm`` runs on the layer norm kernels, in both directions; a subclass with a forward of its own and a
+    module under autocast are called as they are."""
     from .mlp import mlp_module_forward
     from .norm import layer_norm_module_forward
     mlp, norm = decoder_layer.mlp, decoder_layer.post_attention_layernorm
     is_layer_norm = isinstance(norm, nn.LayerNorm)
+    if is_layer_norm and type(norm).forward is nn.LayerNorm.forward and not torch.is_autocast_enabled("cuda"):
+        layer_norm = lambda h: layer_norm_module_forward(norm, h)
+    else:
+        layer_norm = norm
     is_moe = hasattr(mlp, "gate") and hasattr(mlp, "experts")
     block = (lambda x, res=None: layer_forward(mlp, x, res)) if is_moe else (lambda x, res=None: mlp_module_forward(mlp, x))
     bf16_out = bool(getattr(decoder_layer, "_bf16_moe_out", False))
@@ -363,7 +368,7 @@ def ffn_forward(decoder_layer, hidden_states: torch.Tensor) -> torch.Tensor:
     if needs_grad or not plain:
         shape = hidden_states.shape
         if is_layer_norm:
-            x = layer_norm_module_forward(norm, hidden_states)
+            x = layer_norm(hidden_states)
         elif hidden_states.is_cuda and norm.weight.dtype == hidden_states.dtype:
             x = _RMSNormFunction.apply(hidden_states.reshape(-1, shape[-1]).contiguous(), norm.weight,
                                        norm.variance_epsilon).view(shape)
@@ -378,7 +383,7 @@ def ffn_forward(decoder_layer, hidden_states: torch.Tensor) -> torch.Tensor:
     if is_moe and not is_layer_norm and fused_ffn_applies(mlp, hidden_states, norm):
         return layer_forward(mlp, hidden_states, fused_norm=(norm.weight, float(norm.variance_epsilon)))
     if is_layer_norm:
-        x = layer_norm_module_forward(norm, hidden_states)
+        x = layer_norm(hidden_states)
     else:
         flat = hidden_states.reshape(-1, shape[-1]).contiguous()
         x = Fn.rmsnorm_forward(flat, norm.weight, norm.variance_epsilon).view(shape)

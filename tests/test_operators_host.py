@@ -197,3 +197,26 @@ def test_muon_skips_empty_parameters():
     p = torch.nn.Parameter(torch.zeros(4, 0))
     p.grad = torch.zeros(4, 0)
     bibo_b200.Muon([p]).step()
+
+
+def test_feed_forward_calls_a_layer_norm_with_a_forward_of_its_own(monkeypatch):
+    from bibo_b200 import mlp, norm
+    from bibo_b200.moe import ffn_forward
+    monkeypatch.setattr(mlp, "mlp_module_forward", lambda m, x, residual=None: x if residual is None else x + residual)
+    monkeypatch.setattr(norm, "layer_norm_module_forward", lambda m, x: torch.full_like(x, 7))
+
+    class Doubled(torch.nn.LayerNorm):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    h = torch.randn(3, 8)
+    for grad in (True, False):
+        for cls, want in ((torch.nn.LayerNorm, lambda m: torch.full_like(h, 7)), (Doubled, lambda m: m(h))):
+            dl = torch.nn.Module()
+            dl.mlp, dl.post_attention_layernorm = torch.nn.Module(), cls(8)
+            with torch.set_grad_enabled(grad):
+                assert torch.equal(ffn_forward(dl, h), h + want(dl.post_attention_layernorm))
+            if cls is torch.nn.LayerNorm:
+                with monkeypatch.context() as m, torch.set_grad_enabled(grad):
+                    m.setattr(torch, "is_autocast_enabled", lambda *a: True)
+                    assert torch.equal(ffn_forward(dl, h), h + dl.post_attention_layernorm(h))
