@@ -327,7 +327,7 @@ dispatch_kernel(const uint8_t* __restrict__ x, int64_t x_stride_bytes, const int
   }
 }
 
-// weights are fp32 or the rows' type
+// weights are fp32 or bf16, whatever the rows are
 __device__ __forceinline__ float load_weight(const void* w, int is_bf16, int64_t i) {
   return is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]) : static_cast<const float*>(w)[i];
 }
@@ -505,7 +505,8 @@ static int dispatch_check(const char* what, int64_t n_tokens, int hidden, int n_
   if (n_experts < 1 || n_experts > DP_MAX_EXPERTS) return fail(BIBO_ERR_UNSUPPORTED, "%s: n_experts=%d (1..%d)", what, n_experts, DP_MAX_EXPERTS);
   if (top_k < 1 || top_k > DP_MAX_TOP_K) return fail(BIBO_ERR_UNSUPPORTED, "%s: top_k=%d (1..%d)", what, top_k, DP_MAX_TOP_K);
   if (align < 1 || align > 1024) return fail(BIBO_ERR_UNSUPPORTED, "%s: align=%d (1..1024)", what, align);
-  if (n_tokens < 0 || n_tokens * top_k > (1ll << 30)) return fail(BIBO_ERR_UNSUPPORTED, "%s: %lld slots", what, (long long)n_tokens * top_k);
+  if (n_tokens < 0 || n_tokens > (1ll << 30) / top_k)
+    return fail(BIBO_ERR_UNSUPPORTED, "%s: %lld tokens of %d slots", what, (long long)n_tokens, top_k);
   return BIBO_OK;
 }
 static unsigned dispatch_grid(int64_t warps) { return (unsigned)((warps + DW - 1) / DW); }

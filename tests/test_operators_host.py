@@ -30,7 +30,7 @@ def test_c_entry_points_refuse_bad_arguments():
     assert lib.bibo_moe_dispatch_plan(None, 4, 10, 6, 64, 1, p, None) == -1 and b"null" in err()
     assert lib.bibo_moe_dispatch_plan(p, 2, 10, 6, 64, 1, p, None) == -1 and b"indices of 2" in err()
     for n, k, e, a in ((-1, 6, 64, 1), (10, 0, 64, 1), (10, 33, 64, 1), (10, 6, 0, 1), (10, 6, 1025, 1), (10, 6, 64, 0),
-                       (10, 6, 64, 1025), (1 << 28, 6, 64, 1)):
+                       (10, 6, 64, 1025), (1 << 28, 6, 64, 1), (1 << 59, 32, 64, 1)):
         assert lib.bibo_moe_dispatch_plan(p, 4, n, k, e, a, p, None) == -4
         assert lib.bibo_moe_dispatch_rows_cap(n, k, e, a) == -1 and lib.bibo_moe_dispatch_plan_words(n, k, e, a) == -1
         assert lib.bibo_moe_dispatch_fwd(p, 64, p, n, 64, k, e, a, F, p, None) == -4
