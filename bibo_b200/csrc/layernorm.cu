@@ -793,16 +793,23 @@ template <typename T, typename W>
 static int layernorm_fwd_t(const void* x, int64_t x_stride, const void* weight, const void* bias, float eps, int64_t n_rows,
                            int hidden, void* out, float* mean, float* rstd, cudaStream_t st) {
   const int ve = ln_access(hidden, sizeof(T), sizeof(W), n_rows > 1 ? x_stride : 0, 0, x, out, nullptr, weight, bias);
-  // threads, 16-byte pieces a thread, rows a group, blocks an SM.  bf16 rows with fp32 parameters, measured: 32768 x 2048 47.5 us
-  // (0.86 of the copy rate; 256 threads of 8 columns: 56.6), 32768 x 1024 25.5 us (0.80; 128 threads of 8: 31.9), 16384 x 4096 48 us.
-  // Below eight rows an SM a ring has nothing to run ahead of.
+  // Threads of 16 columns, as few as cover the row in steps of 1.5 and 1.33 (idle ones cost issue slots: 2560 columns on 256 threads
+  // ran at 0.67 of the copy rate, on 192 at 0.91); pieces of 16 bytes a thread, rows a group, blocks an SM.  bf16 rows with
+  // fp32 parameters, 537 MB read and written, of the copy rate: 1024 0.83, 1280 0.89, 2048 0.85, 2560 0.91, 4096 0.93, 5120 0.85,
+  // 7168 0.91; fp32 0.85 to 0.91.  Longer fp32 rows need no ring (0.91 to 0.95; 0.85 with it).  Below eight rows an SM a
+  // ring has nothing to run ahead of.
   if (ve * sizeof(T) == 16 && n_rows > 8 * (int64_t)sm_count()) {
     constexpr int VE = 16 / sizeof(T), C16 = 16 / VE;                 // pieces of 16 bytes for 16 columns a thread
 #define BIBO_LN_RING(...) return layernorm_fwd_ring<T, W, __VA_ARGS__>(x, x_stride, weight, bias, eps, n_rows, hidden, out, mean, rstd, st)
-    if (hidden > 512 && hidden <= 1024) BIBO_LN_RING(64, C16, 4, 8);
-    if (hidden > 1024 && hidden <= 2048) BIBO_LN_RING(128, C16, 4, 3);
-    if (hidden > 2048 && hidden <= 4096) BIBO_LN_RING(256, C16, 2, 2);
-    if (hidden > 4096 && hidden * (int)sizeof(T) <= 16384) BIBO_LN_RING(512, C16, 2, 1);
+    if (hidden > 512 && hidden <= 64 * 16) BIBO_LN_RING(64, C16, 4, 8);
+    if (hidden > 64 * 16 && hidden <= 96 * 16) BIBO_LN_RING(96, C16, 4, 4);
+    if (hidden > 96 * 16 && hidden <= 128 * 16) BIBO_LN_RING(128, C16, 4, 3);
+    if (hidden > 128 * 16 && hidden <= 192 * 16) BIBO_LN_RING(192, C16, 4, 3);
+    if (hidden > 192 * 16 && hidden <= 256 * 16) BIBO_LN_RING(256, C16, 2, 2);
+    if constexpr (sizeof(T) == 2) {
+      if (hidden > 256 * 16 && hidden <= 384 * 16) BIBO_LN_RING(384, C16, 4, 1);
+      if (hidden > 384 * 16 && hidden <= 512 * 16) BIBO_LN_RING(512, C16, 4, 1);
+    }
 #undef BIBO_LN_RING
   }
   if constexpr (sizeof(T) == 2) {
@@ -875,14 +882,21 @@ static int layernorm_bwd_pick(const void* x, int64_t x_stride, const void* dy, i
   *done = true;
   if constexpr (VE * sizeof(T) == 16) {
     constexpr int C8 = 8 / VE, C16 = 16 / VE;    // pieces of 16 bytes for 8 and 16 columns a thread
-    // threads, pieces a thread, rows a group, blocks an SM.  bf16 rows with fp32 weight, measured: 32768 x 2048 73 us (0.84 of the
-    // copy rate; two rows a group: 79, 128 threads of 16 columns: 79), 32768 x 1024 46 us (0.67), 16384 x 4096 77 us (0.80).
+    constexpr int RB = VE / 4;                   // rows a group of the same bytes in both types
+    // Threads, pieces a thread, rows a group, blocks an SM: as few threads as cover the row, as in the forward.  bf16 rows with fp32
+    // weight, 805 MB read and written, of the copy rate: 768 0.82, 1024 0.91, 1280 0.81, 1536 0.89, 2048 0.85, 2560 0.88 (256 threads: 0.69),
+    // 4096 0.89 (two rows a group: 0.67, registers), 5120 0.87 (512 threads: 0.69), 8192 0.87; fp32 0.85 to 0.96 (rows of 5120 and
+    // more without a ring: 0.63).
 #define BIBO_LN_RING(...)                                                                                                     \
   return layernorm_bwd_ring<T, W, __VA_ARGS__>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, partial, dweight, dbias, parts, st)
-    if (hidden > 512 && hidden <= 1024) BIBO_LN_RING(128, C8, 4, 4);
-    if (hidden > 1024 && hidden <= 2048) BIBO_LN_RING(256, C8, 4, 2);
-    if (hidden > 2048 && hidden <= 4096) BIBO_LN_RING(256, C16, 1, 2);
-    if (hidden > 4096 && hidden * (int)sizeof(T) <= 16384) BIBO_LN_RING(512, C16, 1, 1);
+    if (hidden > 512 && hidden <= 96 * 8) BIBO_LN_RING(96, C8, 4, 5);
+    if (hidden > 96 * 8 && hidden <= 128 * 8) BIBO_LN_RING(128, C8, 4, 4);
+    if (hidden > 128 * 8 && hidden <= 192 * 8) BIBO_LN_RING(192, C8, 2, 4);
+    if (hidden > 192 * 8 && hidden <= 256 * 8) BIBO_LN_RING(256, C8, 4, 2);
+    if (hidden > 128 * 16 && hidden <= 192 * 16) BIBO_LN_RING(192, C16, RB, 3);
+    if (hidden > 192 * 16 && hidden <= 256 * 16) BIBO_LN_RING(256, C16, 1, 2);
+    if (hidden > 256 * 16 && hidden <= 384 * 16) BIBO_LN_RING(384, C16, RB, 1);
+    if (hidden > 384 * 16 && hidden <= 512 * 16) BIBO_LN_RING(512, C16, 1, 1);
 #undef BIBO_LN_RING
   }
 #define BIBO_LN_BWD(NT, CH, R)                                                                                              \

@@ -100,6 +100,22 @@ def test_many_aligned_rows(n, h, dtype, wtype, pad):
     _compare(x, dy, w, b, 1e-5)
 
 
+@pytest.mark.parametrize("n,h", [(1190, 768), (1203, 776), (1185, 1280), (1201, 1536), (1188, 1544), (1300, 2560), (1187, 2880), (1190, 3584),
+                                 (1186, 5120), (1189, 6144), (1200, 6152), (1185, 7168)])
+@pytest.mark.parametrize("dtype,wtype,pad", [(BF, FP, 0), (BF, BF, 8), (FP, FP, 4)])
+def test_widths_between_the_powers_of_two(n, h, dtype, wtype, pad):
+    x, dy, w, b = _inputs(n, h, dtype, wtype, True, pad, n + h)
+    _compare(x, dy, w, b, 1e-5)
+
+
+@pytest.mark.parametrize("n,h", [(60001, 640), (50002, 1000), (50003, 1280), (30002, 2048), (20011, 2560), (20003, 3584), (12001, 5120),
+                                 (9002, 8192)])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_rows_that_go_round_the_ring_many_times(n, h, dtype):
+    x, dy, w, b = _inputs(n, h, dtype, FP, True, 0, n + h)
+    _compare(x, dy, w, b, 1e-5)
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("pad", [1, 3, 4, 8, 24])
 @pytest.mark.parametrize("h", [64, 2048, 321])
