@@ -399,6 +399,8 @@ dispatch_combine_kernel(const T* __restrict__ ys, const void* __restrict__ weigh
   };
   int c = c_lo;
   for (; c + 32 * U <= c_hi; c += 32 * U) block(c + lane, std::integral_constant<int, U>(), true);
+  if constexpr (U > 2)
+    for (; c + 64 <= c_hi; c += 64) block(c + lane, std::integral_constant<int, 2>(), true);
   for (; c < c_hi; c += 32) block(c + lane, std::integral_constant<int, 1>(), c + lane < c_hi);
 }
 
