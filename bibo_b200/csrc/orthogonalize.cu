@@ -34,7 +34,7 @@ constexpr int NS_MAX_PARTS = 256;                // partial sums of squares per 
 
 // ---- products ----------------------------------------------------------------------------------------------------
 // 256 x 256 tiles: a CTA pair runs tcgen05.mma.cta_group::2 (256 x 256 x 16), each CTA staging its 128 rows of A and its half of
-// B's rows, five stages of 32 KB.  Warps: 0 loads, 1 products (pair leader), 2 loads the sources of the drain and stores its
+// B's rows, four or five stages of 32 KB.  Warps: 0 loads, 1 products (pair leader), 2 loads the sources of the drain and stores its
 // results, 4-11 drain (two warps per quarter of the rows, 32 columns each: with one, a scheduler has nothing to run while its
 // warp waits, and a sub-tile took 1600 cycles).  Results leave in sub-tiles of 64 columns through slots of 16 KB (32 KB where
 // values come or go in two halves): source halves in, result halves out, in place.
@@ -113,7 +113,7 @@ template <int MODE, bool TALL> struct NsOps {
 };
 
 struct NsBars {                                  // barriers and flags in shared memory
-  uint64_t *full, *empty, *tfull, *tempty, *sfull, *cfull, *pfull;   // [stages], [stages], [2], [2], [4], [4], [1]
+  uint64_t *full, *empty, *tfull, *tempty, *sfull, *cfull, *pfull;   // [stages], [stages], [2], [2], [6], [6], [1]
   uint32_t* tmem_slot;
   volatile int* abort_flag;
   __device__ explicit NsBars(unsigned char* smem) {
@@ -122,15 +122,15 @@ struct NsBars {                                  // barriers and flags in shared
     tfull = empty + NS_STAGES;
     tempty = tfull + 2;                                      // pair leader: the drain warps of both CTAs
     sfull = tempty + 2;                                      // a slot's sources have landed (and its last store has left)
-    cfull = sfull + 4;                                       // a slot's results are written
-    pfull = cfull + 4;                                       // the other pairs' partial sums have landed
+    cfull = sfull + 6;                                       // a slot's results are written
+    pfull = cfull + 6;                                       // the other pairs' partial sums have landed
     tmem_slot = reinterpret_cast<uint32_t*>(pfull + 1);
     abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   }
   __device__ __forceinline__ void init() const {
     for (int s = 0; s < NS_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int b = 0; b < 2; ++b) { mbar_init(&tfull[b], 1); mbar_init(&tempty[b], 2 * NS_DRAIN / 32); }
-    for (int b = 0; b < 4; ++b) { mbar_init(&sfull[b], 1); mbar_init(&cfull[b], NS_DRAIN); }
+    for (int b = 0; b < 6; ++b) { mbar_init(&sfull[b], 1); mbar_init(&cfull[b], NS_DRAIN); }
     mbar_init(pfull, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -261,8 +261,9 @@ __device__ __forceinline__ unsigned char* ns_smem() {
   return reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
 }
 
-// Many tiles: persistent pairs, 2 x 256 accumulator columns, so the drain of a tile runs under the next one's products.
-template <int MODE, bool TALL>
+// Many tiles: persistent pairs, 2 x 256 accumulator columns, so the drain of a tile runs under the next one's products.  STAGES of 32 KB, the
+// rest of the 224 KB are slots.
+template <int MODE, bool TALL, int STAGES>
 __global__ void __launch_bounds__(NS_THREADS, 1)
 ns_product_kernel(const __grid_constant__ NsArgs p) {
   unsigned char* smem = ns_smem();
@@ -283,15 +284,15 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
   tc_fence_after();
   const uint32_t tmem_base = *s.tmem_slot;
   pdl_wait();
-  const int halves = p.has_lo || p.out_lo ? 2 : 1, slots = 4 / halves, slot_bits = slots == 4 ? 2 : 1;
-  auto slot_at = [&](int64_t u) { return smem + NS_OFF_SLOT + (int)(u & (slots - 1)) * halves * C_SUB; };
+  const int halves = p.has_lo || p.out_lo ? 2 : 1, slots = (2 * NS_STAGES + 4 - 2 * STAGES) / halves;
+  auto slot_at = [&](int i) { return smem + 2 * STAGES * A_BYTES + i * halves * C_SUB; };
 
   if (warp == 0) {
     if (elect_one()) {
       PipeState ps;
       bool ok = true;
       for (int64_t w = w0; w < p.n_work && ok; w += dw)
-        ok = ns_produce<MODE, TALL>(smem, p, s, ns_decode<MODE>(w, p), 0, p.k_blocks, pr, 0, ps);
+        ok = ns_produce<MODE, TALL, STAGES>(smem, p, s, ns_decode<MODE>(w, p), 0, p.k_blocks, pr, 0, ps);
     }
   } else if (warp == 1) {
     if (pr == 0 && elect_one()) {
@@ -301,7 +302,7 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
       for (int64_t w = w0; w < p.n_work; w += dw) {
         if (!mbar_wait<true>(&s.tempty[acc], acc_phase ^ 1, s.abort_flag)) break;
         tc_fence_after();
-        if (!ns_multiply<MODE, TALL>(smem, s, ns_decode<MODE>(w, p), 0, p.k_blocks, tmem_base + acc * NS_T, 3, ps)) break;
+        if (!ns_multiply<MODE, TALL, STAGES>(smem, s, ns_decode<MODE>(w, p), 0, p.k_blocks, tmem_base + acc * NS_T, 3, ps)) break;
         umma_commit_cg2_mc(&s.tfull[acc], 3);
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1;
@@ -317,30 +318,33 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
         y = t.i * NS_T + pr * BM;
         return x < p.cols && y < p.rows;
       };
-      auto source = [&](int64_t u) {
+      auto source = [&](int64_t u, int slot) {
         if (u >= n_sub) return;
-        uint64_t* bar = &s.sfull[u & (slots - 1)];
+        uint64_t* bar = &s.sfull[slot];
         NsTile t;
         int x, y;
         if (!p.has_s || !place(u, t, x, y)) { mbar_arrive(bar); return; }
         mbar_expect_tx(bar, p.has_lo ? 2 * C_SUB : C_SUB);
-        tma_load_3d(slot_at(u), &p.s_hi, bar, x, y, t.b);
-        if (p.has_lo) tma_load_3d(slot_at(u) + C_SUB, &p.s_lo, bar, x, y, t.b);
+        tma_load_3d(slot_at(slot), &p.s_hi, bar, x, y, t.b);
+        if (p.has_lo) tma_load_3d(slot_at(slot) + C_SUB, &p.s_lo, bar, x, y, t.b);
       };
-      for (int u = 0; u < slots; ++u) source(u);
+      for (int u = 0; u < slots; ++u) source(u, u);
+      int slot = 0;
+      uint32_t phase = 0;
       for (int64_t u = 0; u < n_sub; ++u) {
-        if (!mbar_wait(&s.cfull[u & (slots - 1)], (uint32_t)(u >> slot_bits) & 1u, s.abort_flag)) break;
+        if (!mbar_wait(&s.cfull[slot], phase, s.abort_flag)) break;
         NsTile t;
         int x, y;
         if (place(u, t, x, y)) {
-          tma_store_3d(&p.c_hi, slot_at(u), x, y, t.b);
-          if (p.out_lo) tma_store_3d(&p.c_lo, slot_at(u) + C_SUB, x, y, t.b);
+          tma_store_3d(&p.c_hi, slot_at(slot), x, y, t.b);
+          if (p.out_lo) tma_store_3d(&p.c_lo, slot_at(slot) + C_SUB, x, y, t.b);
           tma_store_commit();
         }
         if (u + slots < n_sub) {
           tma_store_wait_read();
-          source(u + slots);
+          source(u + slots, slot);
         }
+        if (++slot == slots) { slot = 0; phase ^= 1; }
       }
       tma_store_wait_all();
     }
@@ -349,9 +353,8 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
     const int h = (warp - 4) >> 2;
     const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
     const bool poison = p.out_bf16 && *p.status != 0;                 // an earlier product gave up: no number is left to stand
-    int acc = 0;
-    uint32_t acc_phase = 0;
-    int64_t u = 0;
+    int acc = 0, slot = 0;
+    uint32_t acc_phase = 0, phase = 0;
     bool ok = true;
     for (int64_t w = w0; w < p.n_work && ok; w += dw) {
       const NsScale c = ns_scale<MODE>(p, ns_decode<MODE>(w, p).b, poison);
@@ -360,10 +363,10 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
       __syncwarp();
       tc_fence_after();
 #pragma unroll 1
-      for (int g = 0; g < 4; ++g, ++u) {
+      for (int g = 0; g < 4; ++g) {
         float r[32];
         tmem_ld32(lane_addr + acc * NS_T + g * 64 + h * 32, reinterpret_cast<uint32_t*>(r));
-        ok = mbar_wait(&s.sfull[u & (slots - 1)], (uint32_t)(u >> slot_bits) & 1u, s.abort_flag);
+        ok = mbar_wait(&s.sfull[slot], phase, s.abort_flag);
         __syncwarp();
         tmem_ld_wait();
         if (g == 3) {
@@ -372,9 +375,10 @@ ns_product_kernel(const __grid_constant__ NsArgs p) {
           if (lane == 0) mbar_arrive_cluster_addr(map_to_cta(&s.tempty[acc], 0));
         }
         if (!ok) break;
-        ns_finish(p, c, r, slot_at(u), row, h);
+        ns_finish(p, c, r, slot_at(slot), row, h);
         fence_proxy_async_smem();
-        mbar_arrive(&s.cfull[u & (slots - 1)]);
+        mbar_arrive(&s.cfull[slot]);
+        if (++slot == slots) { slot = 0; phase ^= 1; }
       }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
@@ -861,6 +865,12 @@ template <int MODE, bool TALL, int S> static int ns_split_resident(int* clusters
 template <int MODE, bool TALL, int S> static int ns_launch_split(const NsArgs& p, cudaStream_t st) {
   return ns_start(ns_split_kernel<MODE, TALL, S>, dim3((unsigned)p.n_work * 2 * S), NS_THREADS, NS_SMEM, 2 * S, st, p);
 }
+template <int MODE, bool TALL, int STAGES> static int ns_launch_pairs(const NsArgs& p, cudaStream_t st) {
+  static DeviceOnce once;
+  const int rc = ns_attributes(once, ns_product_kernel<MODE, TALL, STAGES>);
+  return rc ? rc : ns_start(ns_product_kernel<MODE, TALL, STAGES>, dim3(2 * (unsigned)std::min<int64_t>(sm_count() / 2, p.n_work)),
+                            NS_THREADS, NS_SMEM, 2, st, p);
+}
 template <int MODE, bool TALL> static int ns_launch(NsArgs& p, int64_t batch, int k_dim, cudaStream_t st) {
   p.m_tiles = (p.rows + NS_T - 1) / NS_T;
   p.n_tiles = (p.cols + NS_T - 1) / NS_T;
@@ -896,10 +906,9 @@ template <int MODE, bool TALL> static int ns_launch(NsArgs& p, int64_t batch, in
   if (rc) return rc;
   if (p.n_work <= four) return ns_launch_split<MODE, TALL, 4>(p, st);
   if (p.n_work <= two) return ns_launch_split<MODE, TALL, 2>(p, st);
-  static DeviceOnce once;
-  rc = ns_attributes(once, ns_product_kernel<MODE, TALL>);
-  return rc ? rc : ns_start(ns_product_kernel<MODE, TALL>, dim3(2 * (unsigned)std::min<int64_t>(sm_count() / 2, p.n_work)), NS_THREADS,
-                            NS_SMEM, 2, st, p);
+  // Short k: a tile's products are over before its drain, which then wants slots more than the products want stages.  All steps of
+  // 64 x 2048 x 512: 773 us with four stages, 805 with five; of 64 x 1024 x 2048 (k = 1024 and more) 2195 against 2170.
+  return p.k_blocks <= 8 ? ns_launch_pairs<MODE, TALL, NS_STAGES - 1>(p, st) : ns_launch_pairs<MODE, TALL, NS_STAGES>(p, st);
 }
 template <int MODE> static int ns_product(NsArgs& p, int tall, int64_t batch, int k_dim, cudaStream_t st) {
   return tall ? ns_launch<MODE, true>(p, batch, k_dim, st) : ns_launch<MODE, false>(p, batch, k_dim, st);
