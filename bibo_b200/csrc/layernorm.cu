@@ -902,12 +902,28 @@ static int layernorm_bwd_pick(const void* x, int64_t x_stride, const void* dy, i
 #define BIBO_LN_BWD(NT, CH, R)                                                                                              \
   return layernorm_bwd_v<T, W, VE, NT, CH, R>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, partial, dweight, dbias, parts, st)
   if (vecs <= 64) BIBO_LN_BWD(64, 1, 8);
-  if (vecs <= 128) BIBO_LN_BWD(128, 1, 4);
-  if (vecs <= 256) BIBO_LN_BWD(256, 1, 4);
-  if (vecs <= 512) BIBO_LN_BWD(256, 2, 2);
-  if (vecs <= 1024) BIBO_LN_BWD(512, 2, 2);
-  if (vecs <= 2048) BIBO_LN_BWD(512, 4, VE < 4 ? 2 : 1);
-  if constexpr (VE < 8) {
+  if constexpr (VE * sizeof(T) == 16) {          // what the rings leave
+    if constexpr (VE == 4) {
+      if (vecs <= 128) BIBO_LN_BWD(128, 1, 4);
+      if (vecs <= 4096) BIBO_LN_BWD(512, 8, 1);
+    } else {
+      if (vecs <= 2048) BIBO_LN_BWD(512, 4, 1);
+    }
+  } else {
+    // Narrow accesses: the issue slots bound, so few threads with many columns each (a row sum costs a thread the same whatever it
+    // adds up), while the registers hold the group.  30000 rows, fp32 at odd strides / bf16 pairs, us (floor), with 256 or 512 threads
+    // before: 301 columns 26 (16), 35; 777 56 (43), 77; 1531 103 (84), 130; bf16 1530 81 (42), 107; 2050 116 (56), 168.
+    constexpr int R2 = VE == 2 ? 1 : 2;
+    if (vecs <= 128) BIBO_LN_BWD(64, 2, 8);
+    if (vecs <= 256) BIBO_LN_BWD(64, 4, 8);
+    if (vecs <= 512) BIBO_LN_BWD(128, 4, 4);
+    if (vecs <= 768) BIBO_LN_BWD(192, 4, R2);
+    if (vecs <= 1024) BIBO_LN_BWD(256, 4, R2);
+    if (vecs <= 1536) BIBO_LN_BWD(384, 4, 1);
+    if (vecs <= 2048) BIBO_LN_BWD(512, 4, 1);
+    if constexpr (VE == 2) {
+      if (vecs <= 384 * 8) BIBO_LN_BWD(384, 8, 1);
+    }
     if (vecs <= 4096) BIBO_LN_BWD(512, 8, 1);
   }
 #undef BIBO_LN_BWD
