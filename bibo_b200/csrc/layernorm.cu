@@ -308,6 +308,119 @@ layernorm_bwd_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restr
   }
 }
 
+// Backward of short rows: G lanes per row, a block of 256 threads walks over 256 / G rows at a time and R such sets, so a row's sums cross
+// lanes only.  The lanes' weight and bias gradients are joined over the block's rows at the end, in a fixed order.  (With a block per
+// row group, 592 blocks of two warps were all that the partial sums allow: 400000 x 128 bf16 took 208 us, 67 this way; x 64 203 and 37.)
+constexpr int LN_N = 256;
+template <typename T, typename W, int VE, int G, int CH, int R>
+__global__ void __launch_bounds__(LN_N)
+layernorm_bwd_short_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ dy, int64_t dy_stride,
+                           const W* __restrict__ weight, const float* __restrict__ mean_in, const float* __restrict__ rstd_in,
+                           int64_t n_rows, int hidden, T* __restrict__ dx, float* __restrict__ partial, W* __restrict__ dweight,
+                           W* __restrict__ dbias) {
+  using X = LnVec<T, VE>;
+  using V = typename X::V;
+  constexpr int GROUPS = LN_N / G;
+  __shared__ float red[2][GROUPS][G * CH * VE];
+  const int lane = threadIdx.x % G, group = threadIdx.x / G, vecs = hidden / VE;
+  tc::pdl_launch_next();                   // layernorm_dparam_kernel may take its place beside this one and wait
+  const float inv = 1.f / (float)hidden;
+  const int64_t total = (int64_t)gridDim.x * GROUPS, first = (int64_t)blockIdx.x * GROUPS + group;
+  float w[CH][VE], dw[CH][VE], db[CH][VE];
+#pragma unroll
+  for (int q = 0; q < CH; ++q) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) { w[q][i] = 1.f; dw[q][i] = db[q][i] = 0.f; }
+    if (weight != nullptr && q * G + lane < vecs) ln_param<W, VE>(weight, q * G + lane, w[q]);
+  }
+  for (int64_t base = 0; base < n_rows; base += total * R) {     // the same number of turns for every lane
+    V xv[R][CH], gv[R][CH];
+    float mean[R], rstd[R], a[R], b[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + r * total + first;
+      const bool in = row < n_rows;
+      const V* xs = reinterpret_cast<const V*>(x + (in ? row : 0) * x_stride);
+      const V* gs = reinterpret_cast<const V*>(dy + (in ? row : 0) * dy_stride);
+      mean[r] = in ? mean_in[row] : 0.f;
+      rstd[r] = in ? rstd_in[row] : 0.f;
+#pragma unroll
+      for (int q = 0; q < CH; ++q) {
+        const int c = q * G + lane;
+        if (in && c < vecs) { xv[r][q] = __ldcs(xs + c); gv[r][q] = __ldcs(gs + c); }
+        else { xv[r][q] = V{}; gv[r][q] = V{}; }                 // adds nothing anywhere
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      a[r] = b[r] = 0.f;
+#pragma unroll
+      for (int q = 0; q < CH; ++q) {
+        float f[VE], g[VE];
+        X::unpack(xv[r][q], f);
+        X::unpack(gv[r][q], g);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          const float z = (f[i] - mean[r]) * rstd[r], gw = g[i] * w[q][i];
+          a[r] += gw;
+          b[r] = fmaf(gw, z, b[r]);
+          dw[q][i] = fmaf(g[i], z, dw[q][i]);
+          db[q][i] += g[i];
+        }
+      }
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        a[r] += __shfl_xor_sync(0xffffffffu, a[r], o);
+        b[r] += __shfl_xor_sync(0xffffffffu, b[r], o);
+      }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = base + r * total + first;
+      if (row >= n_rows) continue;
+      V* ds = reinterpret_cast<V*>(dx + row * hidden);
+      const float m0 = a[r] * inv, m1 = b[r] * inv;
+#pragma unroll
+      for (int q = 0; q < CH; ++q) {
+        const int c = q * G + lane;
+        if (c >= vecs) continue;
+        float f[VE], g[VE];
+        X::unpack(xv[r][q], f);
+        X::unpack(gv[r][q], g);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          const float z = (f[i] - mean[r]) * rstd[r];
+          f[i] = rstd[r] * (fmaf(g[i], w[q][i], -m0) - z * m1);
+        }
+        ds[c] = X::pack(f);
+      }
+    }
+  }
+  if (partial == nullptr && (gridDim.x > 1 || (dweight == nullptr && dbias == nullptr))) return;
+#pragma unroll
+  for (int q = 0; q < CH; ++q)
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      red[0][group][(q * G + lane) * VE + i] = dw[q][i];
+      red[1][group][(q * G + lane) * VE + i] = db[q][i];
+    }
+  __syncthreads();
+  for (int j = threadIdx.x; j < 2 * hidden; j += LN_N) {
+    const int which = j >= hidden, c = j - which * hidden;
+    float s = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) s += red[which][g][c];
+    if (gridDim.x > 1) {
+      partial[(int64_t)blockIdx.x * 2 * hidden + j] = s;
+    } else {                                       // the only block: its sums are the gradients
+      W* dst = which ? dbias : dweight;
+      if (dst != nullptr) dst[c] = from_f32<W>(s);
+    }
+  }
+}
+
 // Backward of 16-byte aligned rows: the same walk, with the rows brought into shared memory by bulk copies several groups ahead
 // (a ring of `stages` groups, about 100 KB in flight per block whatever the registers hold), and z and dy*w of the group kept in
 // registers between the sums and the result.  Arithmetic is in pairs (two fp32 per instruction).  32768 x 2048: 104 us with loads
@@ -873,6 +986,21 @@ static int layernorm_bwd_ring(const void* x, int64_t x_stride, const void* dy, i
   return BIBO_OK;
 }
 
+template <typename T, typename W, int VE, int G, int CH, int R>
+static int layernorm_bwd_short(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
+                               const float* mean, const float* rstd, int64_t n_rows, int hidden, void* dx, float* partial,
+                               void* dweight, void* dbias, int* parts, cudaStream_t st) {
+  int64_t grid = n_rows <= LN_ONE_BLOCK ? 1 : (n_rows + LN_N / G - 1) / (LN_N / G);
+  if (grid > 4 * (int64_t)sm_count()) grid = 4 * (int64_t)sm_count();
+  if (grid > LN_MAX_PARTS) grid = LN_MAX_PARTS;
+  layernorm_bwd_short_kernel<T, W, VE, G, CH, R><<<(unsigned)grid, LN_N, 0, st>>>(
+      static_cast<const T*>(x), x_stride, static_cast<const T*>(dy), dy_stride, static_cast<const W*>(weight), mean, rstd, n_rows,
+      hidden, static_cast<T*>(dx), partial, static_cast<W*>(dweight), static_cast<W*>(dbias));
+  BIBO_CHECK_LAUNCH("layernorm_bwd_short_kernel");
+  *parts = (int)grid;
+  return BIBO_OK;
+}
+
 // columns per thread and rows per group: as many loads in flight as the registers hold beside the 2 CH VE column sums
 template <typename T, typename W, int VE>
 static int layernorm_bwd_pick(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, const void* weight,
@@ -901,10 +1029,16 @@ static int layernorm_bwd_pick(const void* x, int64_t x_stride, const void* dy, i
   }
 #define BIBO_LN_BWD(NT, CH, R)                                                                                              \
   return layernorm_bwd_v<T, W, VE, NT, CH, R>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, partial, dweight, dbias, parts, st)
-  if (vecs <= 64) BIBO_LN_BWD(64, 1, 8);
+#define BIBO_LN_SHORT(G, CH, R)                                                                                             \
+  return layernorm_bwd_short<T, W, VE, G, CH, R>(x, x_stride, dy, dy_stride, weight, mean, rstd, n_rows, hidden, dx, partial, dweight, dbias, parts, st)
   if constexpr (VE * sizeof(T) == 16) {          // what the rings leave
+    // lanes a row, accesses a lane, rows a turn (bf16: two 41, four 37, eight 48 us at 400000 x 64; fp32: 53, 57, 59)
+    if (vecs <= 8) BIBO_LN_SHORT(8, 1, VE / 2);
+    if (vecs <= 16) BIBO_LN_SHORT(16, 1, VE / 2);
+    if (vecs <= 32) BIBO_LN_SHORT(32, 1, VE / 2);
+    if (vecs <= 64) BIBO_LN_SHORT(32, 2, 1);
     if constexpr (VE == 4) {
-      if (vecs <= 128) BIBO_LN_BWD(128, 1, 4);
+      if (vecs <= 128) BIBO_LN_SHORT(32, 4, 1);
       if (vecs <= 4096) BIBO_LN_BWD(512, 8, 1);
     } else {
       if (vecs <= 2048) BIBO_LN_BWD(512, 4, 1);
@@ -914,8 +1048,11 @@ static int layernorm_bwd_pick(const void* x, int64_t x_stride, const void* dy, i
     // adds up), while the registers hold the group.  30000 rows, fp32 at odd strides / bf16 pairs, us (floor), with 256 or 512 threads
     // before: 301 columns 26 (16), 35; 777 56 (43), 77; 1531 103 (84), 130; bf16 1530 81 (42), 107; 2050 116 (56), 168.
     constexpr int R2 = VE == 2 ? 1 : 2;
-    if (vecs <= 128) BIBO_LN_BWD(64, 2, 8);
-    if (vecs <= 256) BIBO_LN_BWD(64, 4, 8);
+    if (vecs <= 8) BIBO_LN_SHORT(8, 1, 4);
+    if (vecs <= 32) BIBO_LN_SHORT(32, 1, 2);
+    if (vecs <= 64) BIBO_LN_SHORT(32, 2, 2);
+    if (vecs <= 128) BIBO_LN_SHORT(32, 4, 2);
+    if (vecs <= 256) BIBO_LN_SHORT(32, 8, 1);
     if (vecs <= 512) BIBO_LN_BWD(128, 4, 4);
     if (vecs <= 768) BIBO_LN_BWD(192, 4, R2);
     if (vecs <= 1024) BIBO_LN_BWD(256, 4, R2);
@@ -927,6 +1064,7 @@ static int layernorm_bwd_pick(const void* x, int64_t x_stride, const void* dy, i
     if (vecs <= 4096) BIBO_LN_BWD(512, 8, 1);
   }
 #undef BIBO_LN_BWD
+#undef BIBO_LN_SHORT
   *done = false;
   return BIBO_OK;
 }

@@ -108,6 +108,15 @@ def test_widths_between_the_powers_of_two(n, h, dtype, wtype, pad):
     _compare(x, dy, w, b, 1e-5)
 
 
+@pytest.mark.parametrize("n", [1, 16, 17, 1031, 40003])
+@pytest.mark.parametrize("h", [2, 8, 12, 40, 64, 66, 100, 128, 131, 200, 256, 260, 392, 512])
+@pytest.mark.parametrize("dtype,wtype,pad", [(BF, FP, 0), (BF, BF, 3), (FP, FP, 0), (FP, FP, 1)])
+def test_short_rows(n, h, dtype, wtype, pad):
+    """Several rows a warp: every number of lanes and accesses, row counts that leave the last turn short, one block and many."""
+    x, dy, w, b = _inputs(n, h, dtype, wtype, True, pad, n + h)
+    _compare(x, dy, w, b, 1e-5)
+
+
 @pytest.mark.parametrize("n,h", [(60001, 640), (50002, 1000), (50003, 1280), (30002, 2048), (20011, 2560), (20003, 3584), (12001, 5120),
                                  (9002, 8192)])
 @pytest.mark.parametrize("dtype", [BF, FP])
