@@ -674,6 +674,14 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch
     if stats.shape != (2, n):
         raise RuntimeError(f"the forward kept {stats.shape[1]} rows, x has {n}")
     dev = x.device
+    if stats.dtype != torch.float32 or stats.device != dev or not stats.is_contiguous() or wtype not in (x.dtype, torch.float32):
+        raise RuntimeError(f"saved is not what layernorm_forward kept for x: statistics {stats.dtype} on {stats.device}, "
+                           f"parameters {wtype} beside {x.dtype} on {dev}")
+    if weight is not None:
+        _need_cuda(weight, "weight")
+        if weight.dim() != 1 or weight.shape[0] != hidden or weight.device != dev or weight.dtype != wtype:
+            raise RuntimeError(f"weight must be the forward's, {wtype} [{hidden}] on {dev}, got {weight.dtype} {tuple(weight.shape)} "
+                               f"on {weight.device}")
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     make = x.new_empty if n else x.new_zeros                   # sums over no rows
     dweight = make(hidden, dtype=wtype) if weight is not None and need_dweight else None

@@ -1,0 +1,50 @@
+"""Calls of the operators beside the block that have to be refused, or answered otherwise, before anything is launched."""
+import pytest
+import torch
+
+
+class _FakeCuda(torch.Tensor):
+    """A tensor that says it is on a GPU, for the checks that come before any launch."""
+
+    @property
+    def is_cuda(self):
+        return True
+
+
+def _fake(t):
+    return t.as_subclass(_FakeCuda)
+
+
+def _zeros(*shape, **kw):
+    return _fake(torch.zeros(*shape, **kw))
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The names of the kernels' entry points that a test's calls would have launched."""
+    from bibo_b200 import functional as Fn
+    names = []
+    monkeypatch.setattr(Fn, "_launch", lambda name, dev, *args: names.append(name))
+    return names
+
+
+def test_layernorm_backward_refuses_a_weight_that_is_not_the_forwards(launches):
+    """The kernel reads [H] elements of the forward's parameter type behind the weight's address."""
+    from bibo_b200 import functional as Fn
+    x, dy = _zeros(4, 64), _zeros(4, 64)
+    stats = _zeros(2, 4)
+    bad = [_zeros(64, dtype=torch.bfloat16), _zeros(8), _zeros(65), _zeros(1, 64), _zeros(128)[::2], torch.zeros(64)]
+    for weight in bad:
+        with pytest.raises(RuntimeError, match="weight"):
+            Fn.layernorm_backward(dy, x, weight, (stats, torch.float32))
+    half = _zeros(4, 64, dtype=torch.bfloat16)
+    for wtype, other in ((torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32)):
+        with pytest.raises(RuntimeError, match="weight must be the forward's"):
+            Fn.layernorm_backward(half, half, _zeros(64, dtype=other), (stats, wtype))
+    for saved in ((stats.double(), torch.float32), (_zeros(4, 2).t(), torch.float32), (stats, torch.bfloat16)):
+        with pytest.raises(RuntimeError, match="not what layernorm_forward kept"):
+            Fn.layernorm_backward(dy, x, None, saved)
+    assert launches == []
+    Fn.layernorm_backward(dy, x, _zeros(64), (stats, torch.float32))
+    Fn.layernorm_backward(half, half, _zeros(64, dtype=torch.bfloat16), (stats, torch.bfloat16))
+    assert launches == ["bibo_moe_layernorm_bwd"] * 2
