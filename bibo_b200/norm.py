@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from . import functional as Fn
@@ -33,9 +34,13 @@ class _LayerNormFunction(torch.autograd.Function):
 
 
 def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5) -> torch.Tensor:
-    """Differentiable layer norm of x [..., H] over H; ``weight`` / ``bias`` [H] are optional, fp32 or of x's dtype."""
+    """Differentiable layer norm of x [..., H] over H; ``weight`` / ``bias`` [H] are optional, fp32 or of x's dtype.  Reverse mode
+    only: inputs with a forward-mode tangent are refused."""
     if x.dim() < 1:
         raise RuntimeError("layer_norm takes a tensor of at least one dimension")
+    # without a reverse-mode gradient no autograd function stands between the tangent and the kernel, which would drop it
+    if any(t is not None and unpack_dual(t).tangent is not None for t in (x, weight, bias)):
+        raise NotImplementedError("bibo_b200: layer_norm has no forward-mode derivative")
     rows = x.reshape(-1, x.shape[-1])
     if rows.shape[1] > 1 and rows.stride(1) != 1 or rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]:
         rows = rows.contiguous()

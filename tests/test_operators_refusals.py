@@ -48,3 +48,22 @@ def test_layernorm_backward_refuses_a_weight_that_is_not_the_forwards(launches):
     Fn.layernorm_backward(dy, x, _zeros(64), (stats, torch.float32))
     Fn.layernorm_backward(half, half, _zeros(64, dtype=torch.bfloat16), (stats, torch.bfloat16))
     assert launches == ["bibo_moe_layernorm_bwd"] * 2
+
+
+def test_layer_norm_refuses_forward_mode_tangents(launches):
+    """The kernel fills a fresh tensor: a tangent would be lost without a word."""
+    import bibo_b200
+    from torch.autograd import forward_ad
+    frozen = bibo_b200.BiBoLayerNorm(8).requires_grad_(False)
+    value, tangent = torch.randn(3, 8), torch.randn(3, 8)
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(value, tangent)
+        w = forward_ad.make_dual(torch.ones(8), torch.randn(8))
+        for call in (lambda: bibo_b200.layer_norm(x), lambda: frozen(x), lambda: bibo_b200.layer_norm(value, w),
+                     lambda: bibo_b200.layer_norm(value, torch.ones(8), w), lambda: bibo_b200.BiBoLayerNorm(8)(x)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(frozen, (value,), (tangent,))
+    assert launches == []
