@@ -23,6 +23,7 @@
 // Symmetric products (G, F, T, R, the second G) are computed and stored on and below the diagonal's 256 x 256 tiles only; an
 // operand tile above it is read as the transposed tile below it, as an MN-major operand.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "orthogonalize_common.cuh"
@@ -972,6 +973,60 @@ static int64_t ns_chunk(int64_t batch, int rows, int cols) {
   return std::max<int64_t>(1, std::min<int64_t>({batch, (2ll << 30) / one, 32768}));
 }
 
+// ---- ranges of the polynomials -----------------------------------------------------------------------------------------
+// The singular values of x_0 lie in [0, 1], and an odd polynomial of them is continuous, so the magnitudes after a step fill
+// [0, M] with M its largest magnitude: each step's range is exact.  What is stored as f16 times 2^12 has to stay below 16.
+constexpr double NS_LIMIT = 15.8, NS_LIMIT_X = 3.97;             // of matrices, and of an x whose Gram matrix is formed (x^2 < 15.8)
+struct NsRange { double lo, hi; double magnitude() const { return std::max(-lo, hi); } };
+// b z + c z^2 over z in [0, top^2]
+static NsRange ns_range_factor(double b, double c, double top) {
+  const double z = top * top, end = z * (b + c * z);
+  NsRange r{std::min(0.0, end), std::max(0.0, end)};
+  const double at = c != 0 ? -b / (2 * c) : 0, v = at * (b + c * at);
+  if (at > 0 && at < z) { r.lo = std::min(r.lo, v); r.hi = std::max(r.hi, v); }
+  return r;
+}
+// the largest |a s + b s^3 + c s^5| over s in [0, top]
+static double ns_range_x(double a, double b, double c, double top) {
+  double most = 0;
+  auto see = [&](double z) {                     // z = s^2
+    if (z > 0 && z <= top * top) most = std::max(most, std::sqrt(z) * std::abs(a + z * (b + c * z)));
+  };
+  see(top * top);
+  if (c != 0) {                                  // a + 3 b z + 5 c z^2 = 0
+    const double d = 9 * b * b - 20 * a * c;
+    if (d >= 0) { see((-3 * b + std::sqrt(d)) / (10 * c)); see((-3 * b - std::sqrt(d)) / (10 * c)); }
+  } else if (b != 0) {
+    see(-a / (3 * b));
+  }
+  return most;
+}
+// The first step that leaves the range (-1: none).  joint: the first two steps may be one, with a step behind them.
+static int ns_check_steps(int steps, const float* co, bool* joint) {
+  double top = 1;
+  *joint = steps >= 3 && co[0] * co[0] <= 14.f && co[0] * co[3] <= 14.f && co[0] > 0.f && co[3] > 0.f;
+  for (int s = 0; s < steps; ++s) {
+    const double a = co[3 * s], b = co[3 * s + 1], c = co[3 * s + 2];
+    const NsRange f = ns_range_factor(b, c, top);
+    const double next = ns_range_x(a, b, c, top);
+    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c) || !(f.magnitude() <= NS_LIMIT) ||
+        !(next <= (s + 1 < steps ? NS_LIMIT_X : NS_LIMIT)))
+      return s;
+    if (s == 0 && *joint) {
+      // T = (a1 + F1)^2 - a1^2 and R = (a2 + F2) (a1 + F1) - a1 a2; where the first polynomial stretches (b > 0, say) neither is
+      // bounded by a1 and a2
+      const NsRange f2 = ns_range_factor(co[4], co[5], next);
+      const double l1 = a + f.lo, h1 = a + f.hi, l2 = co[3] + f2.lo, h2 = co[3] + f2.hi;
+      const double r_lo = std::min({l1 * l2, l1 * h2, h1 * l2, h1 * h2}) - a * co[3];
+      const double r_hi = std::max({l1 * l2, l1 * h2, h1 * l2, h1 * h2}) - a * co[3];
+      const double t = std::max(std::max(l1 * l1, h1 * h1) - a * a, a * a);
+      *joint = t <= NS_LIMIT && std::max(-r_lo, r_hi) <= NS_LIMIT;
+    }
+    top = next;
+  }
+  return -1;
+}
+
 static int ns_maps(NsMaps* m, const void* base, int64_t batch, int rows, int cols, int ld) {
   const int rc = make_tmap_f16_3d(&m->r128, base, batch, rows, cols, ld, BM);
   return rc ? rc : make_tmap_f16_3d(&m->r64, base, batch, rows, cols, ld, 64);
@@ -995,6 +1050,12 @@ extern "C" int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batc
   if (batch < 0 || rows < 0 || cols < 0 || rows > 65535 * 32 || cols > 65535 * 32)
     return fail(BIBO_ERR_ARG, "orthogonalize: %lld matrices of %d x %d", (long long)batch, rows, cols);
   if (steps < 1 || steps > 64 || !coefficients_host) return fail(BIBO_ERR_ARG, "orthogonalize: steps=%d (1..64)", steps);
+  if (!(eps >= 0.f)) return fail(BIBO_ERR_ARG, "orthogonalize: eps=%g", eps);
+  bool joint;                                    // the first two steps as one
+  const int wide = ns_check_steps(steps, coefficients_host, &joint);
+  if (wide >= 0)
+    return fail(BIBO_ERR_UNSUPPORTED, "orthogonalize: step %d takes singular values from [0, 1] out of range (below 4 before the last step, "
+                "|b s^2 + c s^4| below 16)", wide);
   if (batch == 0 || rows == 0 || cols == 0) return BIBO_OK;
   const int cluster = ns_small_cluster(batch, rows, cols);
   if (!u || (!workspace && !cluster) || !out) return fail(BIBO_ERR_ARG, "orthogonalize: null pointer");
@@ -1005,8 +1066,6 @@ extern "C" int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batc
   const int tall = rows > cols, size = dtype == BIBO_F32 ? 4 : 2;
   const int64_t chunk = ns_chunk(batch, rows, cols);
   const float* co = coefficients_host;
-  // the first two steps as one, where their joint matrices stay in range (|T| <= a1^2, |R| <= a1 a2) and a step follows
-  const bool joint = steps >= 3 && co[0] * co[0] <= 14.f && co[0] * co[3] <= 14.f && co[0] > 0.f && co[3] > 0.f;
   if (cluster)
     return ns_small_launch(u, dtype, batch, batch_stride, rows, cols, row_stride, steps, joint, co, eps, cluster, out, st);
   for (int64_t b0 = 0; b0 < batch; b0 += chunk) {

@@ -700,9 +700,13 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7) -> torch.Tensor:
     """Newton-Schulz orthogonalisation of a matrix [m,n] or a stack [..., m, n] (bibo_moe_orthogonalize): with
     x = update / (|update|_F + eps), ``steps`` times x <- a x + (b G + c G^2) x, G = x x^T.  Returns bf16 [..., m, n],
-    contiguous, whatever the update's type (fp32 or bf16).  ``coefficients`` is one (a, b, c) or one for each step; the
-    polynomials a s + b s^3 + c s^5 must keep singular values of at most 1 below 4.  Rows and matrices may be slices
-    of larger ones; any other order (a transposed view, say) is laid out first."""
+    contiguous, whatever the update's type (fp32 or bf16).  ``coefficients`` is one (a, b, c) or one for each step.  The singular
+    values start in [0, 1]; with the values that a step can see, a s + b s^3 + c s^5 must stay below 4 (after the last step
+    below 16) and b s^2 + c s^4 below 16 in magnitude: other coefficients are refused.  Rows and matrices may be slices
+    of larger ones; any other order (a transposed view, say) is laid out first.
+
+    The products take f16 operands and accumulate in fp32, so that the result is off by more than its own rounding to bf16: see
+    the top of csrc/orthogonalize.cu.  |update|_F^2 is summed in fp32."""
     if not update.is_cuda:
         raise RuntimeError(f"update is on {update.device}: the bibo_b200 kernels run only on CUDA devices "
                            "(there is no CPU implementation)")

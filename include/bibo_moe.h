@@ -598,7 +598,8 @@ int bibo_moe_dispatch_combine_bwd(const void* dout, int64_t dout_stride, const v
  * u: `batch` matrices [rows, cols], batch_stride and row_stride elements apart.  x_0 = u / (|u|_F + eps), then `steps`
  * (1..64) times x <- a x + (b G + c G^2) x with G = x x^T (x transposed for tall matrices) and (a, b, c) =
  * coefficients_host[3 * step ..]; out [batch, rows, cols] is bfloat16 and contiguous.  f16 operands, fp32 accumulation;
- * the polynomials must keep the singular values below 4 (|b G + c G^2| below 16).  |u|_F^2 is summed in fp32.
+ * the polynomials must keep the singular values, which start in [0, 1], below 4 before the last step (the result below 16), and
+ * |b s^2 + c s^4| below 16 at every s that a step can see; others are refused.  |u|_F^2 is summed in fp32, eps >= 0.
  * workspace: bibo_moe_orthogonalize_workspace bytes, 128-byte aligned (2 GiB at most, more only where one
  * matrix needs it; 0, and NULL, where the matrices are small enough for shared memory).  If a bounded wait gives up, the whole result of its group of matrices is NaN.   */
 int64_t bibo_moe_orthogonalize_workspace(int64_t batch, int rows, int cols);

@@ -67,3 +67,31 @@ def test_layer_norm_refuses_forward_mode_tangents(launches):
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(frozen, (value,), (tangent,))
     assert launches == []
+
+
+def test_orthogonalize_refuses_polynomials_that_leave_the_range():
+    """x, G and b G + c G^2 are kept as f16 times 2^12, so singular values that start in [0, 1] have to stay below 4 and the factor
+    below 16 in every step that sees them, not in the first one alone."""
+    import ctypes
+    from bibo_b200 import _lib
+    from bibo_b200 import functional as Fn
+    lib = _lib.load()
+
+    def call(*steps, eps=1e-7):
+        flat = (ctypes.c_float * (3 * len(steps)))(*[v for c in steps for v in c])
+        return lib.bibo_moe_orthogonalize(None, 0, 0, 4, 4, 4, _lib.F32, len(steps), flat, eps, None, None, None)   # no matrices
+
+    ns, half = Fn.NEWTON_SCHULZ, (0.5, 0.0, 0.0)
+    assert call(*[ns] * 64) == 0 and call((1.5, -0.5, 0.0)) == 0 and call((1.875, -1.25, 0.375), ns) == 0
+    assert call((1.0, 16.0, -16.0), (0.25, 0.0, 0.0), (1.5, -0.5, 0.0)) == 0            # up to 3.76, factor up to 4
+    assert call((8.25, -23.5, 17.25), (4.0, -3.0, 0.5), (4.0, -3.0, 0.5)) == 0
+    assert call((15.0, 0.0, 0.0)) == 0 and call((15.0, 0.0, 0.0), half) == -4              # the last result need not be squared
+    assert call((16.0, 0.0, 0.0)) == -4
+    assert call((3.9, 0.0, 0.0), ns) == -4 and b"step 1" in lib.bibo_moe_last_error_string()     # factor near 400 at 3.9
+    assert call((1.0, 0.0, -15.9)) == -4 and call((1.0, 64.0, -64.0)) == -4                 # at the end and inside of [0, 1]
+    assert call((0.1, 4.0, 0.0), half) == -4 and call((0.1, 3.8, 0.0), half) == 0
+    assert call((4.0, 16.0, -17.0), half) == -4                                          # 5.8 inside, 3 at s = 1
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for at in range(3):
+            assert call(ns, tuple(bad if i == at else v for i, v in enumerate(ns))) == -4
+    assert call(ns, eps=-1e-7) == -1 and call(ns, eps=float("nan")) == -1 and call(ns, eps=0.0) == 0
