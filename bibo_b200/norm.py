@@ -1,7 +1,8 @@
 """Layer norm on the kernels of ``bibo_moe_layernorm_fwd`` / ``_bwd``.
 
-``BiBoLayerNorm`` is ``torch.nn.LayerNorm`` over the last dimension (same constructor, parameters and state dict) with its
-forward and backward on those kernels; ``bibo_b200.moe.ffn_forward`` takes a decoder layer whose norm is a layer norm.
+``BiBoLayerNorm`` is ``torch.nn.LayerNorm`` over the last dimension (same constructor, parameters, state dict and type under
+autocast: fp32) with its forward and backward on those kernels; ``layer_norm`` keeps its input's type under autocast too.
+``bibo_b200.moe.ffn_forward`` takes a decoder layer whose norm is a layer norm.
 """
 from __future__ import annotations
 
@@ -54,7 +55,10 @@ def layer_norm_module_forward(norm: nn.LayerNorm, x: torch.Tensor) -> torch.Tens
     if len(norm.normalized_shape) != 1 or norm.normalized_shape[0] != x.shape[-1]:
         raise RuntimeError(f"the layer norm kernels normalise the last dimension: normalized_shape {norm.normalized_shape} "
                            f"for an input of {tuple(x.shape)}")
-    return layer_norm(x, norm.weight, norm.bias, norm.eps)
+    weight, bias = norm.weight, norm.bias
+    if torch.is_autocast_enabled("cuda"):           # as torch's: computed and returned in fp32
+        x, weight, bias = (t if t is None or t.dtype == torch.float64 else t.float() for t in (x, weight, bias))
+    return layer_norm(x, weight, bias, norm.eps)
 
 
 class BiBoLayerNorm(nn.LayerNorm):

@@ -95,3 +95,15 @@ def test_orthogonalize_refuses_polynomials_that_leave_the_range():
         for at in range(3):
             assert call(ns, tuple(bad if i == at else v for i, v in enumerate(ns))) == -4
     assert call(ns, eps=-1e-7) == -1 and call(ns, eps=float("nan")) == -1 and call(ns, eps=0.0) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_layer_norm_module_returns_fp32_under_autocast(launches, monkeypatch, dtype):
+    import bibo_b200
+    norm, x = bibo_b200.BiBoLayerNorm(8, dtype=dtype), _zeros(3, 8, dtype=dtype)
+    norm.weight, norm.bias = (torch.nn.Parameter(_fake(p.detach())) for p in (norm.weight, norm.bias))
+    assert norm(x).dtype == dtype
+    monkeypatch.setattr(torch, "is_autocast_enabled", lambda *a: True)
+    with torch.no_grad():
+        assert norm(x).dtype == torch.float32
+    assert norm(x).dtype == torch.float32 and len(launches) == 3
