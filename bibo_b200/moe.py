@@ -342,19 +342,26 @@ class _RMSNormFunction(torch.autograd.Function):
         return dh, dw.to(weight.dtype), None
 
 
+def _is_plain_layer_norm(norm: nn.LayerNorm) -> bool:
+    """Whether a call of the module does no more than ``nn.LayerNorm.forward``: no forward of its own, nobody listening."""
+    return (type(norm).forward is nn.LayerNorm.forward and "forward" not in vars(norm) and
+            not (norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks or
+                 nn.modules.module._has_any_global_hook()))
+
+
 def ffn_forward(decoder_layer, hidden_states: torch.Tensor) -> torch.Tensor:
     """``BiBoDecoderLayer._ffn_forward`` (src/modeling/layers.py:57-67): post-attention RMSNorm, the
     feed-forward block and the residual add.  Inference runs the norm kernel and folds the residual add
     into the combine kernel; with gradients on, norm and block run through their autograd nodes (kernels
     in both directions) and the residual add is torch's.  Written against the reference's attribute
     names (``post_attention_layernorm``, ``mlp``, ``_bf16_moe_out``, ``_bf16_stream``).  A norm that is a
-    ``torch.nn.LayerNorm`` runs on the layer norm kernels, in both directions; a subclass with a forward of its own and a
-    module under autocast are called as they are."""
+    ``torch.nn.LayerNorm`` runs on the layer norm kernels, in both directions; a module with a forward of its own or with hooks
+    and a module under autocast are called as they are."""
     from .mlp import mlp_module_forward
     from .norm import layer_norm_module_forward
     mlp, norm = decoder_layer.mlp, decoder_layer.post_attention_layernorm
     is_layer_norm = isinstance(norm, nn.LayerNorm)
-    if is_layer_norm and type(norm).forward is nn.LayerNorm.forward and not torch.is_autocast_enabled("cuda"):
+    if is_layer_norm and _is_plain_layer_norm(norm) and not torch.is_autocast_enabled("cuda"):
         layer_norm = lambda h: layer_norm_module_forward(norm, h)
     else:
         layer_norm = norm

@@ -32,3 +32,28 @@ def test_layer_norm_module_under_autocast_is_torchs(dtype):
         tol = 1e-5 * float(want.abs().max()) + torch.finfo(want.dtype).eps * want.double().abs()     # two roundings, half a step each
         assert bool(((got.double() - want.double()).abs() <= tol).all())
     assert results[0][0].dtype == torch.float32 and results[0][1].dtype == dtype
+
+
+def _decoder(norm, block="mlp", dtype=torch.bfloat16):
+    from bibo_b200 import BiBoMLP, BiBoMoELayer, MoEConfig
+    dl = torch.nn.Module()
+    cfg = MoEConfig(hidden_size=256, moe_intermediate_size=128, num_routed_experts=64)
+    dl.mlp = BiBoMoELayer(cfg) if block == "moe" else BiBoMLP(cfg, is_expert=True, intermediate_size=256)
+    dl = dl.to(DEV).to(dtype).eval()
+    dl.post_attention_layernorm = norm.to(DEV)
+    return dl
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_feed_forward_fires_the_hooks_of_a_layer_norm(grad):
+    from bibo_b200.moe import ffn_forward
+    torch.manual_seed(2)
+    dl = _decoder(torch.nn.LayerNorm(256, dtype=torch.bfloat16))
+    h, seen = torch.randn(2, 33, 256, device=DEV, dtype=torch.bfloat16), []
+    with torch.set_grad_enabled(grad):
+        want = ffn_forward(dl, h)
+        dl.post_attention_layernorm.register_forward_hook(lambda m, args, out: seen.append(out.detach()))
+        got = ffn_forward(dl, h)
+    # the norm's results may round apart (half a step each of bf16) and pass through the same block: as in the test of the two paths
+    assert len(seen) == 1 and seen[0].shape == h.shape
+    assert float((got.float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())

@@ -107,3 +107,46 @@ def test_layer_norm_module_returns_fp32_under_autocast(launches, monkeypatch, dt
     with torch.no_grad():
         assert norm(x).dtype == torch.float32
     assert norm(x).dtype == torch.float32 and len(launches) == 3
+
+
+def _decoder(norm):
+    dl = torch.nn.Module()
+    dl.mlp, dl.post_attention_layernorm = torch.nn.Module(), norm
+    return dl
+
+
+def test_feed_forward_fires_the_hooks_of_a_layer_norm(monkeypatch):
+    """The kernels are called around the module, so a module with hooks, or with a forward set on it, is called itself."""
+    from bibo_b200 import mlp, norm
+    from bibo_b200.moe import ffn_forward
+    monkeypatch.setattr(mlp, "mlp_module_forward", lambda m, x, residual=None: x if residual is None else x + residual)
+    monkeypatch.setattr(norm, "layer_norm_module_forward", lambda m, x: torch.full_like(x, 7))
+    h, seen = torch.randn(3, 8), []
+    hooks = {
+        "forward": lambda m: m.register_forward_hook(lambda *a: seen.append(1)),
+        "with kwargs": lambda m: m.register_forward_hook(lambda *a: seen.append(1), with_kwargs=True),
+        "pre": lambda m: m.register_forward_pre_hook(lambda *a: seen.append(1)),
+        "backward": lambda m: m.register_full_backward_hook(lambda *a: seen.append(1)),
+        "pre-backward": lambda m: m.register_full_backward_pre_hook(lambda *a: seen.append(1)),
+        "global": lambda m: torch.nn.modules.module.register_module_forward_hook(lambda *a: seen.append(1)),
+    }
+    for kind, register in hooks.items():
+        for grad in (True, False):
+            if "backward" in kind and not grad:
+                continue
+            m = torch.nn.LayerNorm(8)
+            want = h + m(h)
+            handle = register(m)
+            seen.clear()
+            with torch.set_grad_enabled(grad):
+                out = ffn_forward(_decoder(m), h.clone().requires_grad_(grad))
+            if grad:
+                out.sum().backward()
+            handle.remove()
+            assert torch.equal(out, want) and len(seen) >= 1, kind
+            with torch.no_grad():
+                assert torch.equal(ffn_forward(_decoder(m), h), h + 7)          # nobody listens any more
+    m = torch.nn.LayerNorm(8)
+    m.forward = lambda x: 3 * x
+    with torch.no_grad():
+        assert torch.equal(ffn_forward(_decoder(m), h), h + 3 * h)
