@@ -391,6 +391,8 @@ def ffn_forward(decoder_layer, hidden_states: torch.Tensor) -> torch.Tensor:
         return layer_forward(mlp, hidden_states, fused_norm=(norm.weight, float(norm.variance_epsilon)))
     if is_layer_norm:
         x = layer_norm(hidden_states)
+        if x.dtype != hidden_states.dtype:       # under autocast, say: the kernels add a residual of the block's own type only
+            return hidden_states + block(x)
     else:
         flat = hidden_states.reshape(-1, shape[-1]).contiguous()
         x = Fn.rmsnorm_forward(flat, norm.weight, norm.variance_epsilon).view(shape)

@@ -57,3 +57,21 @@ def test_feed_forward_fires_the_hooks_of_a_layer_norm(grad):
     # the norm's results may round apart (half a step each of bf16) and pass through the same block: as in the test of the two paths
     assert len(seen) == 1 and seen[0].shape == h.shape
     assert float((got.float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
+
+
+@pytest.mark.parametrize("block", ["moe", "mlp"])
+def test_feed_forward_of_a_bf16_stream_under_autocast(block):
+    """The norm returns fp32 there; with and without gradients the fp32 block runs and the sum is fp32.  Both run the same kernels
+    or fp32 sums of at most 256 terms in another order: 1e-4 of the largest entry."""
+    from bibo_b200 import BiBoLayerNorm
+    from bibo_b200.moe import ffn_forward
+    torch.manual_seed(3)
+    h = torch.randn(2, 33, 256, device=DEV, dtype=torch.bfloat16)
+    for norm in (BiBoLayerNorm(256), torch.nn.LayerNorm(256)):
+        dl = _decoder(norm, block, torch.float32)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            with torch.no_grad():
+                got = ffn_forward(dl, h)
+            want = ffn_forward(dl, h.clone().requires_grad_()).detach()
+        assert got.dtype == want.dtype == torch.float32
+        assert float((got - want).abs().max()) <= 1e-4 * float(want.abs().max())

@@ -150,3 +150,30 @@ def test_feed_forward_fires_the_hooks_of_a_layer_norm(monkeypatch):
     m.forward = lambda x: 3 * x
     with torch.no_grad():
         assert torch.equal(ffn_forward(_decoder(m), h), h + 3 * h)
+
+
+def test_feed_forward_adds_a_residual_of_another_type_itself(monkeypatch):
+    """A norm that is called as it is may return another type than the stream's: the blocks' kernels refuse such a residual."""
+    from bibo_b200 import mlp, moe
+    from bibo_b200.moe import ffn_forward
+
+    def block(m, x, residual=None):
+        if residual is not None and residual.dtype != x.dtype:
+            raise RuntimeError(f"residual dtype {residual.dtype} != {x.dtype}")
+        return x if residual is None else x + residual
+
+    class Wide(torch.nn.LayerNorm):
+        def forward(self, x):
+            return super().forward(x.float())
+
+    monkeypatch.setattr(mlp, "mlp_module_forward", block)
+    monkeypatch.setattr(moe, "layer_forward", block)
+    h = torch.randn(3, 8, dtype=torch.bfloat16)
+    for is_moe in (False, True):
+        dl = _decoder(Wide(8))
+        if is_moe:
+            dl.mlp.gate = dl.mlp.experts = None
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                got = ffn_forward(dl, h)
+            assert got.dtype == torch.float32 and torch.equal(got, h + dl.post_attention_layernorm(h))
