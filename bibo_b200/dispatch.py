@@ -1,10 +1,18 @@
 """Differentiable token dispatch and combine for experts that are not this package's own.
 
-    idx, w = router(x)                                     # e.g. BiBoMoERouter; idx [N,k], w [N,k]
+    with torch.no_grad():                                  # x [N,H]; the choice of experts has no gradient ...
+        idx = router(x[None])[0][0]                        # a BiBoMoERouter; its weights, the second result, have none either
+    score = torch.sigmoid(x.float() @ router.gate_proj.weight.float().T).gather(1, idx)
+    w = score / score.sum(1, keepdim=True)                 # ... so the weights [N,k] are formed again where the router trains
     plan = functional.dispatch_plan(idx, n_experts)        # rows of expert e: [plan.offsets[e], plan.offsets[e+1])
     xs = dispatch_tokens(x, plan)                          # [plan.rows, H] in expert order
     ys = my_experts(xs, plan.offsets)                      # any row-wise function of xs
     out = combine_tokens(ys, w, plan)                      # [N,H], gradients to ys and w
+
+Gradients end at the ``w`` that is passed: the routers of this package return weights without a gradient (``BiBoMoELayer`` trains its
+router inside the block's own backward), so a router trains through ``combine_tokens`` only if its weights are computed
+differentiably, as above.  An index beyond the experts counts as an empty slot, in both directions, and is reported by
+``plan.raise_if_failed()`` alone, which waits for the plan.
 
 The gradients are the kernels of ``bibo_b200.functional``: sums over a token's slots run in a fixed order.
 """
@@ -53,5 +61,6 @@ def dispatch_tokens(x: torch.Tensor, plan: Fn.DispatchPlan) -> torch.Tensor:
 
 
 def combine_tokens(ys: torch.Tensor, topk_w: Optional[torch.Tensor], plan: Fn.DispatchPlan) -> torch.Tensor:
-    """out [N,H]: each token's rows of ys [plan.rows, H] summed with its weights topk_w [N,k] (None: plain sum)."""
+    """out [N,H]: each token's rows of ys [plan.rows, H] summed with its weights topk_w [N,k] (None: plain sum).  The gradient of
+    ``topk_w`` goes where autograd finds its history; weights straight from ``BiBoMoERouter`` have none."""
     return _CombineFunction.apply(ys, topk_w, plan)

@@ -75,3 +75,37 @@ def test_feed_forward_of_a_bf16_stream_under_autocast(block):
             want = ffn_forward(dl, h.clone().requires_grad_()).detach()
         assert got.dtype == want.dtype == torch.float32
         assert float((got - want).abs().max()) <= 1e-4 * float(want.abs().max())
+
+
+def test_the_frameworks_router_trains_through_combine_tokens():
+    """The steps at the top of bibo_b200/dispatch.py: the choice from BiBoMoERouter, its weights formed again so that they carry a
+    gradient, against the same in 64 bits.  fp32 throughout: sums of at most 90 x 64 order-1 terms, 1e-4 of the largest entry."""
+    import bibo_b200
+    from bibo_b200 import functional
+    torch.manual_seed(4)
+    n, h, e, k = 90, 64, 16, 3
+    router = bibo_b200.BiBoMoERouter(bibo_b200.MoEConfig(hidden_size=h, num_routed_experts=e, num_experts_per_tok=k)).to(DEV)
+    torch.nn.init.normal_(router.gate_proj.weight, std=0.3)
+    experts = torch.randn(e, h, h, device=DEV) / 8
+    x, c = torch.randn(n, h, device=DEV), torch.randn(n, h, device=DEV)
+    with torch.no_grad():
+        idx, given = (t[0] for t in router(x[None]))
+    score = torch.sigmoid(x.float() @ router.gate_proj.weight.float().T).gather(1, idx)
+    w = score / score.sum(1, keepdim=True)
+    assert float((w.detach() - given).abs().max()) <= 1e-5
+    plan = functional.dispatch_plan(idx, e)
+    xs = bibo_b200.dispatch_tokens(x, plan)
+    off = plan.offsets.tolist()
+    ys = torch.cat([xs[off[i]:off[i + 1]] @ experts[i] for i in range(e)])
+    out = bibo_b200.combine_tokens(ys, w, plan)
+    (out * c).sum().backward()
+    plan.raise_if_failed()
+
+    wr = router.gate_proj.weight.detach().double().requires_grad_()
+    s64 = torch.sigmoid(x.double() @ wr.T).gather(1, idx)
+    w64 = s64 / s64.sum(1, keepdim=True)
+    out64 = sum(w64[:, j:j + 1] * torch.einsum("nh,nhi->ni", x.double(), experts.double()[idx[:, j]]) for j in range(k))
+    (out64 * c.double()).sum().backward()
+    for got, want in ((out.detach(), out64.detach()), (router.gate_proj.weight.grad, wr.grad)):
+        assert float((got.double() - want).abs().max()) <= 1e-4 * float(want.abs().max())
+    assert float(wr.grad.abs().max()) > 0
