@@ -697,6 +697,25 @@ def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 
 
+def _polynomials(steps: int, coefficients):
+    """(a, b, c) of every step, one after the other, as the C ABI takes them."""
+    steps = int(steps)
+    if hasattr(coefficients[0], "__len__"):
+        co = list(coefficients)
+    else:
+        co, steps = [coefficients] * min(max(steps, 0), 65), min(steps, 65)      # more than 64 are refused by the library
+    if steps < 1 or len(co) != steps or any(len(c) != 3 for c in co):
+        raise RuntimeError(f"orthogonalize: {steps} steps need one (a, b, c) or {steps} of them")
+    return (C.c_float * (3 * len(co)))(*[float(v) for c in co for v in c])
+
+
+def check_polynomials(steps: int, coefficients, eps: float) -> None:
+    """Raises RuntimeError where ``orthogonalize`` would refuse these steps, without a GPU."""
+    flat = _polynomials(steps, coefficients)
+    _lib.check(_lib.load().bibo_moe_orthogonalize(None, 0, 0, 1, 1, 1, _lib.F32, len(flat) // 3, C.cast(flat, C.c_void_p), float(eps),
+                                                  None, None, None), "bibo_moe_orthogonalize")
+
+
 def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7) -> torch.Tensor:
     """Newton-Schulz orthogonalisation of a matrix [m,n] or a stack [..., m, n] (bibo_moe_orthogonalize): with
     x = update / (|update|_F + eps), ``steps`` times x <- a x + (b G + c G^2) x, G = x x^T.  Returns bf16 [..., m, n],
@@ -718,19 +737,15 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHU
     if (n > 1 and u.stride(2) != 1) or (m > 1 and u.stride(1) < n) or (u.shape[0] > 1 and u.stride(0) < (m - 1) * u.stride(1) + n):
         u = u.contiguous()
     batch = u.shape[0]
-    steps = int(steps)
-    co = [coefficients] * steps if not hasattr(coefficients[0], "__len__") else list(coefficients)
-    if steps < 1 or len(co) != steps or any(len(c) != 3 for c in co):
-        raise RuntimeError(f"orthogonalize: {steps} steps need one (a, b, c) or {steps} of them")
+    flat = _polynomials(steps, coefficients)
     out = torch.empty(update.shape, dtype=torch.bfloat16, device=update.device)
     if update.numel() == 0:
         return out
     lib = _lib.load()
     words = int(lib.bibo_moe_orthogonalize_workspace(batch, m, n))
     ws = torch.empty(words, dtype=torch.uint8, device=update.device) if words else None
-    flat = (C.c_float * (3 * steps))(*[float(v) for c in co for v in c])
     p = _lib.ptr
-    _launch("bibo_moe_orthogonalize", update.device, p(u), batch, u.stride(0), m, n, u.stride(1), dt, steps,
+    _launch("bibo_moe_orthogonalize", update.device, p(u), batch, u.stride(0), m, n, u.stride(1), dt, len(flat) // 3,
             C.cast(flat, C.c_void_p), float(eps), p(ws), p(out))
     return out
 

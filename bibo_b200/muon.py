@@ -24,14 +24,26 @@ class Muon(torch.optim.Optimizer):
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
                  steps: int = 5, coefficients=Fn.NEWTON_SCHULZ, eps: float = 1e-7):
-        if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0:
-            raise ValueError(f"Muon: lr={lr}, momentum={momentum}, weight_decay={weight_decay}")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
                                       coefficients=coefficients, eps=eps))
-        for group in self.param_groups:
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            lr, momentum, weight_decay = group["lr"], group["momentum"], group["weight_decay"]
+            if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0:
+                raise ValueError(f"Muon: lr={lr}, momentum={momentum}, weight_decay={weight_decay}")
             for p in group["params"]:
                 if p.dim() < 2:
                     raise ValueError(f"Muon takes matrices and stacks of them, got a parameter of shape {tuple(p.shape)}")
+            try:
+                Fn.check_polynomials(group["steps"], group["coefficients"], group["eps"])
+            except RuntimeError as e:
+                raise ValueError(f"Muon: {e}") from None
+        except ValueError:
+            self.param_groups.pop()
+            raise
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
@@ -47,6 +59,11 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        for group in self.param_groups:              # nothing is stepped, and no momentum touched, where something is refused
+            for p in group["params"]:
+                if p.grad is not None and p.numel() and (not p.is_cuda or p.grad.layout != torch.strided or p.is_complex()):
+                    raise RuntimeError(f"Muon: a parameter of shape {tuple(p.shape)} on {p.device} with a gradient of {p.grad.dtype}, "
+                                       f"{p.grad.layout}: it takes dense real ones on CUDA devices (there is no CPU implementation)")
         for group in self.param_groups:
             momentum = group["momentum"]
             for p in group["params"]:
@@ -59,7 +76,7 @@ class Muon(torch.optim.Optimizer):
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 buf = state["momentum_buffer"]
                 buf.mul_(momentum).add_(p.grad)
-                u = torch.add(p.grad, buf, alpha=momentum) if group["nesterov"] else buf
+                u = torch.add(p.grad, buf, alpha=momentum).float() if group["nesterov"] else buf
                 u = Fn.orthogonalize(u.contiguous(), group["steps"], group["coefficients"], group["eps"])
                 if group["weight_decay"]:
                     p.mul_(1 - group["lr"] * group["weight_decay"])

@@ -177,3 +177,40 @@ def test_feed_forward_adds_a_residual_of_another_type_itself(monkeypatch):
             with torch.set_grad_enabled(grad):
                 got = ffn_forward(dl, h)
             assert got.dtype == torch.float32 and torch.equal(got, h + dl.post_attention_layernorm(h))
+
+
+def test_muon_refuses_before_it_changes_anything():
+    import bibo_b200
+    from bibo_b200 import functional as Fn
+    make = lambda **kw: bibo_b200.Muon([torch.nn.Parameter(torch.zeros(4, 6))], **kw)
+    opt = make()
+    for bad, match in ((dict(params=[torch.nn.Parameter(torch.zeros(4))]), "matrices"),
+                       (dict(params=[torch.nn.Parameter(torch.zeros(2, 2))], momentum=1.0), "momentum"),
+                       (dict(params=[torch.nn.Parameter(torch.zeros(2, 2))], steps=65), "steps=65"),
+                       (dict(params=[torch.nn.Parameter(torch.zeros(2, 2))], coefficients=(9.0, 0.0, 0.0)), "out of range")):
+        with pytest.raises(ValueError, match=match):
+            opt.add_param_group(bad)
+        assert len(opt.param_groups) == 1
+    for bad in (dict(steps=0), dict(steps=1 << 40), dict(steps=2, coefficients=[Fn.NEWTON_SCHULZ]), dict(eps=-1.0),
+                dict(coefficients=(1.0, float("nan"), 0.0))):
+        with pytest.raises(ValueError, match="Muon"):
+            make(**bad)
+    # a parameter that is not on a GPU, beside one that says it is: neither has moved afterwards
+    near, far = torch.nn.Parameter(_zeros(4, 6)), torch.nn.Parameter(torch.zeros(4, 6))
+    for p in (near, far):
+        p.grad = torch.ones(4, 6)
+    opt = bibo_b200.Muon([near, far])
+    momentum = torch.full((4, 6), 3.0)
+    opt.state[near]["momentum_buffer"] = momentum
+    with pytest.raises(RuntimeError, match="no CPU implementation"):
+        opt.step()
+    assert bool((momentum == 3).all()) and not opt.state[far]
+
+
+def test_orthogonalize_refuses_step_counts_without_building_them():
+    from bibo_b200 import functional as Fn
+    with pytest.raises(RuntimeError, match="steps=65"):
+        Fn.check_polynomials(1 << 40, Fn.NEWTON_SCHULZ, 1e-7)
+    with pytest.raises(RuntimeError, match="steps need"):
+        Fn.check_polynomials(1 << 40, [Fn.NEWTON_SCHULZ] * 3, 1e-7)
+    Fn.check_polynomials(64, Fn.NEWTON_SCHULZ, 0.0)
