@@ -1121,6 +1121,7 @@ static int layernorm_check(const char* what, int64_t n_rows, int hidden, int dty
   if (wdtype != BIBO_F32 && wdtype != dtype)
     return fail(BIBO_ERR_ARG, "%s: weight dtype=%d beside activations of dtype=%d", what, wdtype, dtype);
   if (hidden < 1) return fail(BIBO_ERR_ARG, "%s: hidden=%d", what, hidden);
+  if (hidden > 1 << 30) return fail(BIBO_ERR_UNSUPPORTED, "%s: hidden=%d", what, hidden);   // column counters pass it by a block
   if (n_rows > 0x7fffffffll) return fail(BIBO_ERR_UNSUPPORTED, "%s: %lld rows", what, (long long)n_rows);
   if (stride < hidden) return fail(BIBO_ERR_ARG, "%s: row stride %lld below hidden=%d", what, (long long)stride, hidden);
   return BIBO_OK;
@@ -1153,6 +1154,8 @@ extern "C" int bibo_moe_layernorm_bwd(const void* x, int64_t x_stride, const voi
   int rc = layernorm_check("layernorm_bwd", n_rows, hidden, dtype, wdtype, n_rows > 1 ? x_stride : hidden);
   if (!rc) rc = layernorm_check("layernorm_bwd", n_rows, hidden, dtype, wdtype, n_rows > 1 ? dy_stride : hidden);
   if (rc) return rc;
+  if ((dweight || dbias) && hidden > 65535 * LN_T)      // the grid of layernorm_bwd_cols_kernel
+    return fail(BIBO_ERR_UNSUPPORTED, "layernorm_bwd: parameter gradients of hidden=%d (%d at most)", hidden, 65535 * LN_T);
   if (n_rows <= 0) return BIBO_OK;      // the caller's dweight / dbias are sums over no rows: it zeroes them itself
   if (!x || !dy || !mean || !rstd || !dx || ((dweight || dbias) && !partial && ln_parts(n_rows) > 0))
     return fail(BIBO_ERR_ARG, "layernorm_bwd: null pointer");

@@ -424,6 +424,8 @@ def experts_forward(x: torch.Tensor, topk_idx: torch.Tensor, topk_w: torch.Tenso
 def _plan_layout(n_tokens: int, top_k: int, n_experts: int, align: int) -> Tuple[int, int, int, int]:
     """(rows, words, word of slot_row, word of row_slot) of a plan of these sizes."""
     lib = _lib.load()
+    if max(top_k, n_experts, align) >= 1 << 31:                  # the C ABI takes 32 bits of them
+        raise RuntimeError(f"dispatch plan: top_k={top_k}, n_experts={n_experts}, align={align}")
     rows = int(lib.bibo_moe_dispatch_rows_cap(n_tokens, top_k, n_experts, align))
     if rows < 0:
         raise RuntimeError("dispatch plan: " + lib.bibo_moe_last_error_string().decode(errors="replace"))
@@ -590,6 +592,8 @@ def _rows(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
     if t.dim() != 2 or t.shape[1] < 1:
         raise RuntimeError(f"{name} must be rows [N, H] with H >= 1, got shape {tuple(t.shape)}")
     n, h = t.shape
+    if h > 1 << 30:
+        raise RuntimeError(f"{name} has rows of {h} elements, the kernels take up to 2^30")
     s0, s1 = t.stride()
     if (s1 != 1 and h > 1) or (s0 < h and n > 1):
         raise RuntimeError(f"{name} must be contiguous within its rows, which may not overlap (strides {t.stride()})")
@@ -733,6 +737,8 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHU
         raise RuntimeError(f"update must be a matrix or a stack of matrices, got shape {tuple(update.shape)}")
     dt = dtype_code(update.dtype)
     m, n = update.shape[-2:]
+    if max(m, n) > 65535 * 32:
+        raise RuntimeError(f"orthogonalize: matrices of {m} x {n}, the kernels take up to {65535 * 32} rows and columns")
     u = update.reshape(-1, m, n) if update.numel() else update.reshape(0, m, n)
     if (n > 1 and u.stride(2) != 1) or (m > 1 and u.stride(1) < n) or (u.shape[0] > 1 and u.stride(0) < (m - 1) * u.stride(1) + n):
         u = u.contiguous()

@@ -214,3 +214,29 @@ def test_orthogonalize_refuses_step_counts_without_building_them():
     with pytest.raises(RuntimeError, match="steps need"):
         Fn.check_polynomials(1 << 40, [Fn.NEWTON_SCHULZ] * 3, 1e-7)
     Fn.check_polynomials(64, Fn.NEWTON_SCHULZ, 0.0)
+
+
+def test_sizes_beyond_32_bits_are_refused_and_not_cut(launches):
+    """The C ABI takes them as 32-bit integers: 2^32 + 8 columns would be eight."""
+    from bibo_b200 import _lib
+    from bibo_b200 import functional as Fn
+    lib = _lib.load()
+    wide = _fake(torch.empty(1, 2 ** 32 + 8, device="meta"))
+    with pytest.raises(RuntimeError, match="up to 2\\^30"):
+        Fn.layernorm_forward(wide)
+    plan = Fn.DispatchPlan(1, 1, 8, 1, "meta")
+    for call in (lambda: Fn.dispatch_forward(wide, plan), lambda: Fn.combine_forward(wide, None, plan),
+                 lambda: Fn.combine_backward(wide, wide, None, plan)):
+        with pytest.raises(RuntimeError, match="up to 2\\^30"):
+            call()
+    for shape in ((2 ** 32 + 4, 8), (8, 2 ** 32 + 4)):
+        with pytest.raises(RuntimeError, match="rows and columns"):
+            Fn.orthogonalize(_fake(torch.empty(shape, device="meta")))
+    for k, e, a in ((2, 2 ** 32 + 8, 1), (2, 8, 2 ** 32 + 1), (2 ** 32 + 2, 8, 1)):
+        with pytest.raises(RuntimeError, match="dispatch plan"):
+            Fn.dispatch_plan(_fake(torch.empty(0, k, dtype=torch.int32, device="meta")), e, a)
+    assert launches == []
+    p = 4096                                                    # never read: refused before the first launch
+    assert lib.bibo_moe_layernorm_fwd(p, 1 << 31, p, p, 1e-5, 4, (1 << 30) + 1, _lib.F32, _lib.F32, p, None, None, None) == -4
+    wide = 65535 * 256 + 1
+    assert lib.bibo_moe_layernorm_bwd(p, wide, p, wide, p, p, p, 4, wide, _lib.F32, _lib.F32, p, p, p, p, None) == -4
