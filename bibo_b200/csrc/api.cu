@@ -230,7 +230,7 @@ int host_pipe(HostPipe** out) {
   return BIBO_OK;
 }
 // Slice lengths: equal slices of about 4096 tokens (a multiple of the router block), at most
-// HOST_MAX_SLICES of them.  A tapered tail (shorter last slices) and 2048 / 3072 / 6144 / 8192-token slices
+// HOST_MAX_SLICES of them.  A tapered tail (shorter last slices) and 2048 / 6144 / 8192-token slices
 // all measured slower.  BIBO_HOST_SLICE_TOKENS overrides the length (0 = one slice, no overlap).
 int host_slices(int64_t n_tokens, int64_t* lens) {
   static const int64_t forced = [] { const char* e = getenv("BIBO_HOST_SLICE_TOKENS"); return e ? atoll(e) : -1; }();

@@ -15,7 +15,7 @@
 namespace bibo {
 
 // words of the plan buffer: offsets [E+1], counts [E], status, then (16-byte aligned) slot_row [slots], row_slot [rows] and, for
-// more slots than one block sorts, scratch [blocks][E+1]
+// more slots than one block sorts, scratch: counts [blocks][E], then a flag of each block
 __host__ __device__ inline int64_t dp_off_counts(int E) { return E + 1; }
 __host__ __device__ inline int64_t dp_off_status(int E) { return 2 * (int64_t)E + 1; }
 __host__ __device__ inline int64_t dp_off_slot_row(int E) { return (2 * (int64_t)E + 2 + 3) / 4 * 4; }

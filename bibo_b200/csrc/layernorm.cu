@@ -420,9 +420,10 @@ layernorm_bwd_short_kernel(const T* __restrict__ x, int64_t x_stride, const T* _
   }
 }
 
-// Backward of 16-byte aligned rows: the same walk, with the rows brought into shared memory by bulk copies several groups ahead
-// (a ring of `stages` groups, about 100 KB in flight per block whatever the registers hold), and z and dy*w of the group kept in
-// registers between the sums and the result.  Arithmetic is in pairs (two fp32 per instruction).  32768 x 2048: 104 us with loads
+// Backward of 16-byte aligned rows: the same walk, with the rows brought into shared memory by bulk copies (a ring of one to eight
+// groups in the block's share of 208 KB), and z and dy*w of the group kept in registers between the sums and the result.  Where the
+// share holds one group only (fp32 rows at the wide end of some classes, as 768, 1024 and 2048 columns or 1024 forward) nothing runs
+// ahead inside the block, and the SM's other blocks are what has loads in flight.  Arithmetic is in pairs (two fp32 per instruction).  32768 x 2048: 104 us with loads
 // into registers (57 % of the issue slots, 64 KB in flight an SM), 73 us with the ring.
 __device__ __forceinline__ float2 ln_fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -450,7 +451,7 @@ __device__ __forceinline__ void ln_bulk_load(void* dst, const void* src, uint32_
 
 constexpr int LN_MAX_STAGES = 8;
 // Forward of 16-byte aligned rows, many of them: a block walks over groups of R rows that bulk copies bring into a ring in shared
-// memory several groups ahead; a thread owns CH x VE columns, keeps their parameters in registers and a group's values
+// memory, up to seven groups ahead where the ring holds as many (see above); a thread owns CH x VE columns, keeps their parameters in registers and a group's values
 // between the two sums.  (A warp per row re-reads the parameters from L1 for every row: with fp32 parameters beside bf16 rows
 // that is twice the row's own bytes, and 32768 x 2048 took 54.7 us with L1 at 78 %; two rows a warp, 58 us, lacked loads in flight.)
 template <typename T, typename W, int NT, int CH, int R>

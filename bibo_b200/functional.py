@@ -477,7 +477,7 @@ class DispatchPlan:
 def dispatch_plan(topk_idx: torch.Tensor, n_experts: int, align: int = 1) -> DispatchPlan:
     """Row order of the routing ``topk_idx`` [N,k] (int32 or int64; a negative index is an empty slot, an expert may occur
     more than once in a token).  ``align``: groups start at multiples of it, with rows without a slot behind them.  k up to
-    32, up to 1024 experts, one kernel launch, nothing is read back."""
+    32, up to 1024 experts; one kernel launch up to 8192 slots, two above, nothing is read back."""
     _need_cuda(topk_idx, "topk_idx")
     if topk_idx.dim() != 2 or topk_idx.dtype not in (torch.int32, torch.int64):
         raise RuntimeError(f"topk_idx must be int32 or int64 [N, k], got {topk_idx.dtype} {tuple(topk_idx.shape)}")
@@ -728,8 +728,9 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=NEWTON_SCHU
     below 16) and b s^2 + c s^4 below 16 in magnitude: other coefficients are refused.  Rows and matrices may be slices
     of larger ones; any other order (a transposed view, say) is laid out first.
 
-    The products take f16 operands and accumulate in fp32, so that the result is off by more than its own rounding to bf16: see
-    the top of csrc/orthogonalize.cu.  |update|_F^2 is summed in fp32."""
+    The products take f16 operands and accumulate in fp32.  The result is off by 0.0017-0.0026 (relative, Frobenius, the usual
+    coefficients) where its rounding to bf16 alone is 0.0017, and by up to 0.004 where the short side is below 65 (more below 16:
+    0.005 seen at 12 x 16384, 0.012 at 2 x 2): figures by size at the top of csrc/orthogonalize.cu.  |update|_F^2 is summed in fp32."""
     if not update.is_cuda:
         raise RuntimeError(f"update is on {update.device}: the bibo_b200 kernels run only on CUDA devices "
                            "(there is no CPU implementation)")

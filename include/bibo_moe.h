@@ -601,7 +601,9 @@ int bibo_moe_dispatch_combine_bwd(const void* dout, int64_t dout_stride, const v
  * the polynomials must keep the singular values, which start in [0, 1], below 4 before the last step (the result below 16), and
  * |b s^2 + c s^4| below 16 at every s that a step can see; others are refused.  |u|_F^2 is summed in fp32, eps >= 0.
  * workspace: bibo_moe_orthogonalize_workspace bytes, 128-byte aligned (2 GiB at most, more only where one
- * matrix needs it; 0, and NULL, where the matrices are small enough for shared memory).  If a bounded wait gives up, the whole result of its group of matrices is NaN.   */
+ * matrix needs it; 0, and NULL, where the matrices are small enough for shared memory).  If a bounded wait gives up, what it can have
+ * reached is NaN: its whole group of matrices, or, where it was in the last product (the last step of small matrices), the tiles
+ * (the columns) of the block that gave up.                                                              */
 int64_t bibo_moe_orthogonalize_workspace(int64_t batch, int rows, int cols);
 int bibo_moe_orthogonalize(const void* u, int64_t batch, int64_t batch_stride, int rows, int cols, int64_t row_stride,
                            int dtype, int steps, const float* coefficients_host, float eps, void* workspace, void* out,

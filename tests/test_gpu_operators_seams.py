@@ -56,7 +56,8 @@ def test_feed_forward_fires_the_hooks_of_a_layer_norm(grad):
         got = ffn_forward(dl, h)
     # the norm's results may round apart (half a step each of bf16) and pass through the same block: as in the test of the two paths
     assert len(seen) == 1 and seen[0].shape == h.shape
-    assert float((got.float() - want.float()).abs().max()) <= 2.0 ** -7 * float(want.float().abs().max())
+    got, want = got.detach().float(), want.detach().float()
+    assert float((got - want).abs().max()) <= 2.0 ** -7 * float(want.abs().max())
 
 
 @pytest.mark.parametrize("block", ["moe", "mlp"])
@@ -109,3 +110,21 @@ def test_the_frameworks_router_trains_through_combine_tokens():
     for got, want in ((out.detach(), out64.detach()), (router.gate_proj.weight.grad, wr.grad)):
         assert float((got.double() - want).abs().max()) <= 1e-4 * float(want.abs().max())
     assert float(wr.grad.abs().max()) > 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_muon_steps_parameters_of_every_real_type(dtype, nesterov):
+    """The first step: the momentum is the gradient, u = 1.95 g or g in fp32, and the same kernel call gives the same bits."""
+    import bibo_b200
+    from bibo_b200 import functional
+    torch.manual_seed(5)
+    p = torch.nn.Parameter(torch.randn(40, 24, device=DEV).to(dtype))
+    before = p.detach().clone()
+    p.grad = torch.randn(40, 24, device=DEV).to(dtype)
+    bibo_b200.Muon([p], lr=0.5, nesterov=nesterov).step()
+    u = torch.add(p.grad, p.grad.float(), alpha=0.95).float() if nesterov else p.grad.float()
+    want = before.double() - 0.5 * (40 / 24) ** 0.5 * functional.orthogonalize(u).double()
+    # one sum in the parameter's type, or in fp32 on the way to it: half a step of each
+    tol = (torch.finfo(dtype).eps + 2.0 ** -22) * want.abs() + 2.0 ** -20
+    assert bool(((p.detach().double() - want).abs() <= tol).all())
