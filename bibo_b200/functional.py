@@ -670,8 +670,8 @@ def layernorm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bi
 
 def layernorm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], saved, has_bias: bool = True,
                        need_dweight: bool = True):
-    """Gradients of ``layernorm_forward(..., keep=True)`` (bibo_moe_layernorm_bwd): (dx [N,H], dweight [H] or None without
-    a weight, dbias [H] or None without a bias).  The sums over the rows are taken in a fixed order."""
+    """Gradients of ``layernorm_forward(..., keep=True)`` (bibo_moe_layernorm_bwd) on its x, weight and what it kept: (dx [N,H],
+    dweight [H] or None without a weight, dbias [H] or None without a bias).  The sums over the rows are taken in a fixed order."""
     stats, wtype = saved
     n, hidden, stride = _rows(x, "x")
     dy_stride = _rows_like(dy, "dy", n, hidden, x)

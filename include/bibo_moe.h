@@ -551,7 +551,7 @@ int bibo_moe_rmsnorm_bwd(const void* h, const void* weight, const void* dy, floa
  * feed-forward path.  out = (x - mean) * rstd * weight + bias over each row, rstd = 1/sqrt(var + eps), computed in
  * fp32 and rounded once.  x [N,H] with rows x_stride elements apart (any alignment; 16-byte aligned rows run faster),
  * out [N,H] contiguous; weight / bias [H] or NULL, both of wdtype = dtype or float32.  mean / rstd [N] fp32, both or
- * neither NULL: what the backward reads.                                                                 */
+ * neither NULL: what the backward reads.  hidden <= 2^30 (65535 * 256 for parameter gradients).          */
 int bibo_moe_layernorm_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias, float eps,
                            int64_t n_rows, int hidden, int dtype, int wdtype, void* out, float* mean, float* rstd,
                            void* stream);
